@@ -71,8 +71,8 @@ enum nrs_status {
  * pixels.  A caller who needs f32 arithmetic beyond that asks for FP32. */
 enum nrs_math_mode { NRS_MATH_3XTF32 = 0, NRS_MATH_TF32 = 1, NRS_MATH_FP32 = 2 };
 
-/* Activation fused into a contraction's epilogue. */
-enum nrs_act { NRS_ACT_NONE = 0, NRS_ACT_RELU = 1, NRS_ACT_GELU = 2 };
+/* Activation fused into a contraction's epilogue.  SILU (x / (1 + exp(-x))): of gated layers (nrs_gated_linear_fwd) only. */
+enum nrs_act { NRS_ACT_NONE = 0, NRS_ACT_RELU = 1, NRS_ACT_GELU = 2, NRS_ACT_SILU = 3 };
 
 /* ------------------------------------------------------------- lifecycle -- */
 
@@ -333,6 +333,20 @@ int nrs_dropout_mask(nrs_ctx* ctx, float* mask, size_t count, float p);
 int nrs_rng_seed(nrs_ctx* ctx, uint64_t seed);
 int nrs_rng_offset(nrs_ctx* ctx, uint64_t* offset);
 
+/* Dropout whose mask is never stored (no reference counterpart: dropout.rs:45-48 keeps one): y = x * m (+ residual) and
+ * dx (+)= g * m, where m[i / hw] is the value nrs_dropout_mask gives for the same seed and first counter block, made again
+ * in each pass.  hw == 1: a value per element; hw = h*w: one per (sample, channel) plane.  residual may be NULL; y may be x
+ * or residual, and dx may be g.  The values multiply, also where m is 0: an infinity or NaN there gives NaN, as
+ * nrs_mask_mul does.  Draws are arguments: a captured call replays the same ones, and a forward pass is repeated by
+ * repeating its arguments.
+ * nrs_rng_take takes the counter blocks of `count` mask values out of the context's stream, as nrs_dropout_mask would
+ * (under data parallelism: this process's samples' part of the global draw). */
+int nrs_rng_take(nrs_ctx* ctx, size_t count, uint64_t* seed, uint64_t* first_block);
+int nrs_dropout_fwd(nrs_ctx* ctx, const float* x, const float* residual, float* y, size_t total, int hw, float p,
+                    uint64_t seed, uint64_t first_block);
+int nrs_dropout_bwd(nrs_ctx* ctx, const float* g, float* dx, size_t total, int hw, float p, uint64_t seed,
+                    uint64_t first_block, int accumulate);
+
 /* ------------------------------------------------------- input pipeline -- */
 
 /* `augment` of examples/cifar_cuda.rs:146-169 on a resident batch x[n,c,h,w] -> y:
@@ -382,6 +396,32 @@ int nrs_attention_fwd(nrs_ctx* ctx, const float* q, const float* k, const float*
 int nrs_attention_bwd(nrs_ctx* ctx, const float* q, const float* k, const float* v, const float* probs, const float* dout,
                       float* dq, float* dk, float* dv, int batch, int seq, int heads, int d_head, int acc_q, int acc_k,
                       int acc_v);
+/* RMS norm of every query and key head and the rotation of its position, in one pass (no reference counterpart; the
+ * relative alternative to the added table of src/cuda/nn/positional.rs:18-44).  q: `tokens` rows of heads_q heads of d_head
+ * features, rows ld_q floats apart (a packed projection's row); k the same with heads_k heads.  Per head x:
+ *   z = gamma * x / sqrt(mean(x^2) + eps);   out = z with its first rot_dim features turned, pair by pair, by the angle of
+ *   the token's position: (a, b) -> (a cos - b sin, a sin + b cos); pairs are features (i, i + rot_dim/2), or neighbours
+ *   (2i, 2i+1) when `interleaved`.
+ * gamma_*: [d_head], NULL for ones.  table: nrs_rotary_table's, [max_len][rot_dim/2][cos, sin]; NULL (and rot_dim 0): no
+ * rotation.  positions: int32 per token on the device, NULL for t % seq.  A position outside the table is not looked up: that
+ * token's rows are zeros (and its gradients), and the next nrs_sync / nrs_d2h returns NRS_ERR_ARG.  heads_q or heads_k may
+ * be 0.  d_head up to 1024.  In place (q_out == q with equal strides) is allowed; other overlaps are not.
+ * Backward: g_* are the gradients of the outputs, q and k the forward pass's inputs; writes (accumulate == 0) or adds to dq,
+ * dk, and (accumulate_params) dgamma_q, dgamma_k; each may be NULL.  dq may be g_q (not with accumulate).  The workspace, at
+ * least nrs_qk_norm_rotary_workspace bytes, is used by this call alone: calls that may run at the same time (two captured
+ * graphs) bring one each.  Deterministic. */
+int nrs_rotary_table(nrs_ctx* ctx, float* table, int max_len, int rot_dim, float base);
+int nrs_qk_norm_rotary_fwd(nrs_ctx* ctx, const float* q, int64_t ld_q, const float* k, int64_t ld_k, const float* gamma_q,
+                           const float* gamma_k, const float* table, const int32_t* positions, float* q_out,
+                           int64_t ld_q_out, float* k_out, int64_t ld_k_out, int tokens, int seq, int heads_q, int heads_k,
+                           int d_head, int rot_dim, int max_len, int interleaved, float eps);
+size_t nrs_qk_norm_rotary_workspace(int tokens, int heads_q, int heads_k, int d_head);
+int nrs_qk_norm_rotary_bwd(nrs_ctx* ctx, const float* g_q, int64_t ld_gq, const float* g_k, int64_t ld_gk, const float* q,
+                           int64_t ld_q, const float* k, int64_t ld_k, const float* gamma_q, const float* gamma_k,
+                           const float* table, const int32_t* positions, float* dq, int64_t ld_dq, float* dk, int64_t ld_dk,
+                           float* dgamma_q, float* dgamma_k, int tokens, int seq, int heads_q, int heads_k, int d_head,
+                           int rot_dim, int max_len, int interleaved, float eps, int accumulate, int accumulate_params,
+                           void* workspace, size_t workspace_bytes);
 /* Head split / merge for multi-head attention: to_heads != 0 maps x[batch, s, heads*d_head] to
  * y[batch*heads, s, d_head] (head h = column slice [h*d_head, (h+1)*d_head), exactly the slices
  * src/nn/multihead.rs:94-107 takes one by one); to_heads == 0 is the inverse, i.e. the

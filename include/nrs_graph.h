@@ -91,12 +91,15 @@ int nrs_op_batchnorm_act(nrs_node* x, nrs_node* gamma, nrs_node* beta, nrs_node*
                          float momentum, float eps, int training, int act, nrs_node** out);
 /* dropout (src/cuda/nn/dropout.rs:31-84) and dropout2d (src/cuda/nn/dropout2d.rs:37-).
  * training == 0 hands back the input node itself (one more reference on it).  `mask`
- * NULL draws the mask on the device (nrs_dropout_mask: the context's seed and
- * counter); a resident mask node (one value per element, or per (sample, channel)
+ * NULL draws the mask on the device (the values of nrs_dropout_mask: the context's
+ * seed and counter), again in each pass, without storing it; a resident mask node (one value per element, or per (sample, channel)
  * plane for dropout2d; values 0 or 1/(1-p)) is used as given, which is how a caller
  * replays masks drawn elsewhere. */
 int nrs_op_dropout(nrs_node* x, float p, int training, nrs_node* mask, nrs_node** out);
 int nrs_op_dropout2d(nrs_node* x, float p, int training, nrs_node* mask, nrs_node** out);
+/* residual + dropout(x) in one pass, the residual form of a transformer's sublayers (training == 0: their sum).  Like
+ * nrs_op_dropout without a mask of the caller's, it stores no mask: the backward pass makes it again. */
+int nrs_op_dropout_add(nrs_node* x, nrs_node* residual, float p, int training, nrs_node** out);
 /* Fused x@W+b -> activation and conv+bias -> activation (enum nrs_act). */
 int nrs_op_linear_act(nrs_node* x, nrs_node* w, nrs_node* b, int act, nrs_node** out);
 int nrs_op_conv2d_act(nrs_node* input, nrs_node* weight, nrs_node* bias, int64_t stride, int64_t pad, int act,
@@ -120,6 +123,20 @@ int nrs_op_attention_batch(nrs_node* q, nrs_node* k, nrs_node* v, int causal, nr
 /* MultiHeadAttention::forward_batch(x) with weights [d,d] and no biases. */
 int nrs_op_mha(nrs_node* x, nrs_node* w_q, nrs_node* w_k, nrs_node* w_v, nrs_node* w_o, int64_t num_heads,
                int causal, nrs_node** out);
+/* The rotation table (nrs_rotary_table) as a resident node [max_len, rot_dim] without a gradient, and the norms and
+ * rotations of nrs_qk_norm_rotary_fwd on q [.., seq, heads_q * d] and k [.., seq, heads_k * d] ([tokens, features] or
+ * [batch, seq, features]): two results, each with a backward pass of its own.  gamma_q, gamma_k, table: NULL for none.
+ * positions: HOST array, one per token, checked against the table; NULL: the place in the sequence.  No reference
+ * counterpart. */
+int nrs_rotary_new(nrs_ctx* ctx, int64_t rot_dim, int64_t max_len, float base, nrs_node** table_out);
+int nrs_op_qk_norm_rotary(nrs_node* q, nrs_node* k, nrs_node* gamma_q, nrs_node* gamma_k, nrs_node* table,
+                          const int32_t* positions_host, int64_t heads_q, int64_t heads_k, int interleaved, float eps,
+                          nrs_node** q_out, nrs_node** k_out);
+/* nrs_op_mha whose queries and keys go through nrs_op_qk_norm_rotary (gamma_q, gamma_k: [d / num_heads]) on their way
+ * from the projections to the scores. */
+int nrs_op_mha_rotary(nrs_node* x, nrs_node* w_q, nrs_node* w_k, nrs_node* w_v, nrs_node* w_o, nrs_node* gamma_q,
+                      nrs_node* gamma_k, nrs_node* table, int64_t num_heads, int interleaved, float eps, int causal,
+                      nrs_node** out);
 /* TransformerBlock::forward / forward_no_final_norm.  params: 12 nodes in the
  * order w_q, w_k, w_v, w_o, norm1.gamma, norm1.beta, norm2.gamma, norm2.beta,
  * ff1.weights, ff1.bias, ff2.weights, ff2.bias (the reference's parameters()

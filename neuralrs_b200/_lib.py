@@ -26,7 +26,7 @@ STATUS_NAMES = {0: "NRS_OK", 1: "NRS_ERR_ARG", 2: "NRS_ERR_SHAPE", 3: "NRS_ERR_A
                 5: "NRS_ERR_NCCL", 6: "NRS_ERR_TIMEOUT", 7: "NRS_ERR_UNSUPPORTED"}
 
 MATH_3XTF32, MATH_TF32, MATH_FP32 = 0, 1, 2
-ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 
 
 class NrsError(RuntimeError):

@@ -210,6 +210,7 @@ int nrs_check_device_error(nrs_ctx* ctx) {
   *ctx->err_host = 0;
   if (code == 5)
     return nrs_fail(ctx, NRS_ERR_ARG, "an embedding lookup met a token index outside the vocabulary; that row was read as zeros");
+  if (code == 6) return nrs_fail(ctx, NRS_ERR_ARG, "a rotation met a position outside its table; that token's rows were written as zeros");
   static const char* what[] = {"", "TMA producer waiting for a free ring slot", "UMMA issuer waiting for a filled ring slot",
                                "epilogue waiting for the accumulator", "draining outstanding TMA loads"};
   return nrs_fail(ctx, NRS_ERR_TIMEOUT, "a tensor-core kernel gave up a bounded wait (%s); its output is invalid",

@@ -79,6 +79,76 @@ mask_mul_kernel(const float* __restrict__ a, const float* __restrict__ mask, flo
   }
 }
 
+// Dropout without a mask in memory: out = a * m (+ residual), or out (+)= a * m, with the mask of dropout_mask_kernel made
+// again wherever it is needed.  What a stored mask costs, 4 bytes written and read again in both passes and kept between
+// them, is spent on twenty wide multiplications per block of four instead, which run under the loads.
+//   FOURS: hw == 1, a block's four words serve four neighbouring elements; otherwise element i takes mask value i / hw
+//   VEC:   16-byte accesses (FOURS: aligned tensors; planes: hw a multiple of 4 too, so that a vector has one mask value)
+template <bool FOURS, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+dropout_kernel(const float* a, const float* residual, float* out, size_t total, size_t hw, float p, float scale, uint64_t seed, uint64_t first,
+               int accumulate) {
+  NRS_PDL_PROLOGUE();
+  constexpr int kUnroll = 4;   // vectors of a thread under way together
+  const size_t groups = (FOURS || VEC) ? (total + 3) / 4 : total;
+  const float* add = accumulate ? out : residual;
+  for (size_t base = (size_t)blockIdx.x * (kThreads * kUnroll) + threadIdx.x; base < groups; base += (size_t)gridDim.x * (kThreads * kUnroll)) {
+    float4 v[kUnroll], r[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const size_t b = base + (size_t)u * kThreads;
+      v[u] = r[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (b >= groups) continue;
+      if (VEC && 4 * b + 4 <= total) {
+        v[u] = reinterpret_cast<const float4*>(a)[b];
+        if (add) r[u] = reinterpret_cast<const float4*>(add)[b];
+      } else if (FOURS) {
+        float e[4] = {}, f[4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (4 * b + j < total) { e[j] = a[4 * b + j]; if (add) f[j] = add[4 * b + j]; }
+        v[u] = make_float4(e[0], e[1], e[2], e[3]);
+        r[u] = make_float4(f[0], f[1], f[2], f[3]);
+      } else {
+        v[u].x = a[b];
+        if (add) r[u].x = add[b];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const size_t b = base + (size_t)u * kThreads;
+      if (b >= groups) continue;
+      uint32_t w[4];
+      float4 m;
+      if (FOURS) {
+        nrs_rng::block(seed, first + b, w);
+        m = make_float4(mask_value(w[0], p, scale), mask_value(w[1], p, scale), mask_value(w[2], p, scale), mask_value(w[3], p, scale));
+      } else {
+        const size_t at = VEC ? 4 * b : b, i = (at | hw) >> 32 ? at / hw : (size_t)((uint32_t)at / (uint32_t)hw);
+        nrs_rng::block(seed, first + i / 4, w);
+        const uint32_t k = (uint32_t)i & 3u;
+        const float one = mask_value(k < 2 ? (k == 0 ? w[0] : w[1]) : (k == 2 ? w[2] : w[3]), p, scale);
+        m = make_float4(one, one, one, one);
+      }
+      float4 y = make_float4(v[u].x * m.x, v[u].y * m.y, v[u].z * m.z, v[u].w * m.w);
+      if (add) {   // rounded once, as mask_mul_kernel does (but for the rest of a length that is no multiple of four)
+        if (VEC && 4 * b + 4 > total) y = make_float4(__fadd_rn(r[u].x, y.x), __fadd_rn(r[u].y, y.y), __fadd_rn(r[u].z, y.z), 0.0f);
+        else y = make_float4(fmaf(v[u].x, m.x, r[u].x), fmaf(v[u].y, m.y, r[u].y), fmaf(v[u].z, m.z, r[u].z), fmaf(v[u].w, m.w, r[u].w));
+      }
+      if (VEC && 4 * b + 4 <= total) {
+        reinterpret_cast<float4*>(out)[b] = y;
+      } else if (FOURS) {
+        const float e[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (4 * b + j < total) out[4 * b + j] = e[j];
+      } else {
+        out[b] = y.x;
+      }
+    }
+  }
+}
+
 unsigned ew_blocks(const nrs_ctx* ctx, size_t work_items) {
   const size_t want = (work_items + kThreads - 1) / kThreads;
   const size_t cap = (size_t)ctx->sm_count * 16;
@@ -134,4 +204,50 @@ int nrs_mask_mul(nrs_ctx* ctx, const float* a, const float* mask, float* out, si
   }
   NRS_LAUNCHED(ctx);
   return NRS_OK;
+}
+
+int nrs_rng_take(nrs_ctx* ctx, size_t count, uint64_t* seed, uint64_t* first_block) {
+  NRS_REQUIRE_CTX(ctx);
+  NRS_REQUIRE(ctx, seed && first_block, NRS_ERR_ARG, "nrs_rng_take: null output");
+  uint64_t advance = 0;
+  *seed = ctx->rng_seed;
+  nrs_rng_window(ctx, count, first_block, &advance);   // a data-parallel shard takes its samples' part of the global draw
+  ctx->rng_offset += advance;
+  return NRS_OK;
+}
+
+static int dropout_pass(nrs_ctx* ctx, const char* who, const float* a, const float* residual, float* out, size_t total, int hw, float p,
+                        uint64_t seed, uint64_t first, int accumulate) {
+  NRS_REQUIRE(ctx, p >= 0.0f && p <= 1.0f, NRS_ERR_ARG, "%s: probability %g outside [0,1]", who, (double)p);
+  NRS_REQUIRE(ctx, hw >= 1, NRS_ERR_SHAPE, "%s: bad plane size %d", who, hw);
+  if (total == 0) return NRS_OK;
+  NRS_REQUIRE(ctx, a && out, NRS_ERR_ARG, "%s: null tensor", who);
+  NRS_REQUIRE(ctx, total % (size_t)hw == 0, NRS_ERR_SHAPE, "%s: %zu elements are not whole planes of %d", who, total, hw);
+  NrsDeviceGuard on(ctx);
+  const float scale = 1.0f / (1.0f - p);   // (p == 1: infinite and never used, as in nrs_dropout_mask)
+  const bool aligned = (((uintptr_t)a | (uintptr_t)out | (uintptr_t)residual) & 15) == 0;
+  const size_t groups = hw == 1 || (aligned && hw % 4 == 0) ? (total + 3) / 4 : total;
+  const size_t want = (groups + 4 * kThreads - 1) / (4 * kThreads), cap = (size_t)ctx->sm_count * 16;
+  const unsigned blocks = (unsigned)(want > cap ? cap : want);
+#define NRS_DROPOUT(FOURS_, VEC_)                                                                                                       \
+  NRS_PDL_LAUNCH((dropout_kernel<FOURS_, VEC_>), blocks, kThreads, 0, ctx->stream, a, residual, out, total, (size_t)hw, p, scale, seed, \
+                 first, accumulate)
+  if (hw == 1 && aligned) NRS_DROPOUT(true, true);
+  else if (hw == 1) NRS_DROPOUT(true, false);
+  else if (aligned && hw % 4 == 0) NRS_DROPOUT(false, true);
+  else NRS_DROPOUT(false, false);
+#undef NRS_DROPOUT
+  NRS_LAUNCHED(ctx);
+  return NRS_OK;
+}
+
+int nrs_dropout_fwd(nrs_ctx* ctx, const float* x, const float* residual, float* y, size_t total, int hw, float p, uint64_t seed,
+                    uint64_t first_block) {
+  NRS_REQUIRE_CTX(ctx);
+  return dropout_pass(ctx, __func__, x, residual, y, total, hw, p, seed, first_block, 0);
+}
+
+int nrs_dropout_bwd(nrs_ctx* ctx, const float* g, float* dx, size_t total, int hw, float p, uint64_t seed, uint64_t first_block, int accumulate) {
+  NRS_REQUIRE_CTX(ctx);
+  return dropout_pass(ctx, __func__, g, nullptr, dx, total, hw, p, seed, first_block, accumulate != 0);
 }

@@ -1268,11 +1268,17 @@ NodeP dropout_nd(const NodeP& x, float p, bool training, const NodeP& mask, bool
     if (mask->len() != mask_len) fail(NRS_ERR_SHAPE, (w + ": mask length mismatch").c_str());
     mask_ptr = mask->data;
     out->parents.push_back(mask);   // keeps the caller's mask alive until the backward pass has run
-  } else {
-    float* m = dalloc(ctx, mask_len);
-    out->saved.push_back(m);
-    check(ctx, nrs_dropout_mask(ctx, m, mask_len, p));
-    mask_ptr = m;
+  } else {   // the mask is made again in the backward pass
+    uint64_t seed = 0, first = 0;
+    check(ctx, nrs_rng_take(ctx, mask_len, &seed, &first));
+    check(ctx, nrs_dropout_fwd(ctx, x->data, nullptr, out->data, x->len(), (int)hw, p, seed, first));
+    Node* self = out.get();
+    out->backward_fn = [self, x, hw, p, seed, first]() {
+      if (!x->requires_grad) return;
+      GradTarget t = grad_target(x);
+      check(self->ctx, nrs_dropout_bwd(self->ctx, grad_in(self), t.ptr, x->len(), (int)hw, p, seed, first, t.accumulate));
+    };
+    return out;
   }
   check(ctx, nrs_mask_mul(ctx, x->data, mask_ptr, out->data, x->len(), (int)hw, 0));
   Node* self = out.get();
@@ -1292,6 +1298,33 @@ NodeP dropout(const NodeP& x, float p, bool training, const NodeP& mask) {
 
 NodeP dropout2d(const NodeP& x, float p, bool training, const NodeP& mask) {
   return dropout_nd(x, p, training, mask, true, "cuda dropout2d");
+}
+
+NodeP dropout_add(const NodeP& x, const NodeP& residual, float p, bool training) {
+  require_gpu(x, "cuda dropout_add: input");
+  require_gpu(residual, "cuda dropout_add: residual");
+  if (x->shape != residual->shape) fail(NRS_ERR_SHAPE, "cuda dropout_add: shapes differ");
+  if (x->ctx != residual->ctx) fail(NRS_ERR_ARG, "cuda dropout_add: nodes of different contexts");
+  if (!(p >= 0.0f && p <= 1.0f)) fail(NRS_ERR_ARG, "cuda dropout_add: probability outside [0,1]");
+  if (x->len() == 0) fail(NRS_ERR_SHAPE, "cuda dropout_add: empty input");
+  if (!training) return add(residual, x);
+  nrs_ctx* ctx = x->ctx;
+  uint64_t seed = 0, first = 0;
+  check(ctx, nrs_rng_take(ctx, x->len(), &seed, &first));
+  NodeP out = make_out(ctx, x->shape, {x, residual});
+  check(ctx, nrs_dropout_fwd(ctx, x->data, residual->data, out->data, x->len(), 1, p, seed, first));
+  Node* self = out.get();
+  out->backward_fn = [self, x, residual, p, seed, first]() {
+    nrs_ctx* ctx = self->ctx;
+    const float* g = grad_in(self);
+    const size_t len = self->len();
+    if (x->requires_grad) {
+      GradTarget t = grad_target(x);
+      check(ctx, nrs_dropout_bwd(ctx, g, t.ptr, len, 1, p, seed, first, t.accumulate));
+    }
+    pass_grad(ctx, residual, g, len);
+  };
+  return out;
 }
 
 // dX = dz W^T of a Linear layer.  Where x is the output of another Linear layer with a fused activation and this is

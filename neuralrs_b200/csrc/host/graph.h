@@ -205,6 +205,8 @@ NodeP batchnorm_act(const NodeP& x, const NodeP& gamma, const NodeP& beta, const
 // dropout.rs / dropout2d.rs: evaluation returns `x` itself; `mask` == nullptr draws the mask on the device
 NodeP dropout(const NodeP& x, float p, bool training, const NodeP& mask = nullptr);
 NodeP dropout2d(const NodeP& x, float p, bool training, const NodeP& mask = nullptr);
+// residual + dropout(x) in one pass (evaluation: their sum)
+NodeP dropout_add(const NodeP& x, const NodeP& residual, float p, bool training);
 // Fused variants with no counterpart op in the reference: one kernel for
 // x@W + b followed by an activation, and conv + bias + activation.  Backward is
 // the composition of the unfused backward passes.
@@ -249,10 +251,22 @@ struct PositionalEncoding {           // positional.rs:18-44; the table is compu
   // x: [seq, d] as in the reference, or [batch, seq, d] (table broadcast over the batch).
   NodeP forward(const NodeP& x) const;
 };
+// nrs_rotary_table as a node [max_len, rot_dim] without a gradient.
+NodeP rotary_table(nrs_ctx* ctx, size_t rot_dim, size_t max_len, float base);
+// RMS norm of every head of q and k and the rotation of its position (nrs_qk_norm_rotary_fwd); no reference counterpart.
+struct HeadNorm {
+  NodeP gamma_q, gamma_k, table;      // each may be null
+  bool interleaved = false;
+  float eps = 1e-6f;
+};
+struct QueryKey { NodeP q, k; };
+QueryKey qk_norm_rotary(const NodeP& q, const NodeP& k, size_t heads_q, size_t heads_k, const HeadNorm& norm, const int32_t* positions_host = nullptr);
+
 struct MultiHeadAttention {           // multihead.rs:57-85; no biases
   NodeP w_q, w_k, w_v, w_o;
   size_t d_model = 0, num_heads = 1;
   bool causal = false;                // extension
+  const HeadNorm* head_norm = nullptr;   // of the projected queries and keys (extension)
   NodeP forward_batch(const NodeP& x) const;
 };
 struct TransformerBlock {             // transformer_block.rs:28-60: post-LN, ReLU feed-forward

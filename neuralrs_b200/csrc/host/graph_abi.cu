@@ -284,6 +284,11 @@ int nrs_op_dropout(nrs_node* x, float p, int training, nrs_node* mask, nrs_node*
   return wrap(ctx_of(x), out, [&] { return nrs::cuda::dropout(x->p, p, training != 0, mask ? mask->p : nullptr); });
 }
 
+int nrs_op_dropout_add(nrs_node* x, nrs_node* residual, float p, int training, nrs_node** out) {
+  NODE_OK(x); NODE_OK(residual);
+  return wrap(ctx_of(x), out, [&] { return nrs::cuda::dropout_add(x->p, residual->p, p, training != 0); });
+}
+
 int nrs_op_dropout2d(nrs_node* x, float p, int training, nrs_node* mask, nrs_node** out) {
   NODE_OK(x);
   if (mask) NODE_OK(mask);
@@ -353,6 +358,48 @@ int nrs_op_mha(nrs_node* x, nrs_node* w_q, nrs_node* w_k, nrs_node* w_v, nrs_nod
   if (num_heads < 1 || x->p->shape.size() != 3) return nrs_fail(ctx_of(x), NRS_ERR_SHAPE, "mha: bad heads or input rank");
   return wrap(ctx_of(x), out, [&] {
     nrs::cuda::MultiHeadAttention m{w_q->p, w_k->p, w_v->p, w_o->p, x->p->shape[2], (size_t)num_heads, causal != 0};
+    return m.forward_batch(x->p);
+  });
+}
+
+int nrs_rotary_new(nrs_ctx* ctx, int64_t rot_dim, int64_t max_len, float base, nrs_node** table_out) {
+  NRS_REQUIRE_CTX(ctx);
+  NRS_REQUIRE(ctx, rot_dim > 0 && max_len > 0, NRS_ERR_SHAPE, "nrs_rotary_new: non-positive size");
+  return wrap(ctx, table_out, [&] { return nrs::cuda::rotary_table(ctx, (size_t)rot_dim, (size_t)max_len, base); });
+}
+
+static nrs::cuda::HeadNorm head_norm_of(nrs_node* gamma_q, nrs_node* gamma_k, nrs_node* table, int interleaved, float eps) {
+  return {gamma_q ? gamma_q->p : nullptr, gamma_k ? gamma_k->p : nullptr, table ? table->p : nullptr, interleaved != 0, eps};
+}
+
+int nrs_op_qk_norm_rotary(nrs_node* q, nrs_node* k, nrs_node* gamma_q, nrs_node* gamma_k, nrs_node* table, const int32_t* positions_host,
+                          int64_t heads_q, int64_t heads_k, int interleaved, float eps, nrs_node** q_out, nrs_node** k_out) {
+  NODE_OK(q);
+  NODE_OK(k);
+  nrs_ctx* ctx = ctx_of(q);
+  if (!q_out || !k_out) return nrs_fail(ctx, NRS_ERR_ARG, "null out handle");
+  *q_out = *k_out = nullptr;
+  if (heads_q < 1 || heads_k < 1) return nrs_fail(ctx, NRS_ERR_SHAPE, "qk norm: head counts must be positive");
+  return guarded(ctx, [&] {
+    const nrs::cuda::QueryKey r = nrs::cuda::qk_norm_rotary(q->p, k->p, (size_t)heads_q, (size_t)heads_k,
+                                                            head_norm_of(gamma_q, gamma_k, table, interleaved, eps), positions_host);
+    auto first = std::make_unique<nrs_node>(nrs_node{r.q});
+    *k_out = new nrs_node{r.k};
+    *q_out = first.release();
+  });
+}
+
+int nrs_op_mha_rotary(nrs_node* x, nrs_node* w_q, nrs_node* w_k, nrs_node* w_v, nrs_node* w_o, nrs_node* gamma_q, nrs_node* gamma_k, nrs_node* table,
+                      int64_t num_heads, int interleaved, float eps, int causal, nrs_node** out) {
+  NODE_OK(x);
+  NODE_OK(w_q);
+  NODE_OK(w_k);
+  NODE_OK(w_v);
+  NODE_OK(w_o);
+  if (num_heads < 1 || x->p->shape.size() != 3) return nrs_fail(ctx_of(x), NRS_ERR_SHAPE, "mha: bad heads or input rank");
+  return wrap(ctx_of(x), out, [&] {
+    const nrs::cuda::HeadNorm norm = head_norm_of(gamma_q, gamma_k, table, interleaved, eps);
+    nrs::cuda::MultiHeadAttention m{w_q->p, w_k->p, w_v->p, w_o->p, x->p->shape[2], (size_t)num_heads, causal != 0, &norm};
     return m.forward_batch(x->p);
   });
 }

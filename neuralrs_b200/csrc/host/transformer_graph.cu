@@ -205,6 +205,86 @@ static NodeP permute_heads(const NodeP& x, size_t batch, size_t seq, size_t head
   return out;
 }
 
+NodeP rotary_table(nrs_ctx* ctx, size_t rot_dim, size_t max_len, float base) {
+  if (!ctx) fail(NRS_ERR_ARG, "rotary table: null context");
+  if (rot_dim == 0 || rot_dim > 1024 || max_len == 0 || max_len > 2147483647u) fail(NRS_ERR_SHAPE, "rotary table: bad shape");
+  NodeP table = make_result(ctx, {max_len, rot_dim}, {});
+  table->requires_grad = false;
+  check(ctx, nrs_rotary_table(ctx, table->data, (int)max_len, (int)rot_dim, base));
+  return table;
+}
+
+QueryKey qk_norm_rotary(const NodeP& q, const NodeP& k, size_t heads_q, size_t heads_k, const HeadNorm& norm, const int32_t* positions_host) {
+  for (const NodeP& n : {q, k})
+    if (!n || !n->on_gpu()) fail(NRS_ERR_ARG, "cuda qk norm: input not on GPU");
+  for (const NodeP& n : {k, norm.gamma_q, norm.gamma_k, norm.table}) {
+    if (n && !n->on_gpu()) fail(NRS_ERR_ARG, "cuda qk norm: parameter not on GPU");
+    if (n && n->ctx != q->ctx) fail(NRS_ERR_ARG, "cuda qk norm: nodes of different contexts");
+  }
+  const size_t nd = q->shape.size();
+  if ((nd != 2 && nd != 3) || k->shape.size() != nd || heads_q == 0 || heads_k == 0 || heads_q > 65535 || heads_k > 65535 ||
+      q->shape[nd - 1] % heads_q != 0 || q->shape[nd - 1] == 0)
+    fail(NRS_ERR_SHAPE, "cuda qk norm: inputs must be [tokens, heads * d] or [batch, seq, heads * d]");
+  const size_t seq = q->shape[nd - 2], tokens = nd == 3 ? q->shape[0] * seq : seq, d = q->shape[nd - 1] / heads_q;
+  if (k->shape[nd - 1] != heads_k * d || k->shape[nd - 2] != seq || (nd == 3 && k->shape[0] != q->shape[0]) || tokens > 2147483647u || d > 1024)
+    fail(NRS_ERR_SHAPE, "cuda qk norm: shapes of queries and keys do not match");
+  for (const NodeP& n : {norm.gamma_q, norm.gamma_k})
+    if (n && n->len() != d) fail(NRS_ERR_SHAPE, "cuda qk norm: gamma must have a value per feature of a head");
+  if (norm.table && norm.table->shape.size() != 2) fail(NRS_ERR_SHAPE, "cuda qk norm: the table must be [max_len, rot_dim]");
+  nrs_ctx* ctx = q->ctx;
+  const int rot = norm.table ? (int)norm.table->shape[1] : 0, max_len = norm.table ? (int)norm.table->shape[0] : 0;
+  std::shared_ptr<void> positions;   // on the device, shared by both results
+  if (positions_host && norm.table && tokens) {
+    for (size_t i = 0; i < tokens; ++i)
+      if (positions_host[i] < 0 || positions_host[i] >= max_len) fail(NRS_ERR_ARG, "cuda qk norm: position outside the rotation table");
+    void* p = nullptr;
+    check(ctx, nrs_alloc(ctx, tokens * sizeof(int32_t), 0, &p));
+    positions = std::shared_ptr<void>(p, [ctx](void* q) { nrs_free(ctx, q); });
+    check(ctx, nrs_h2d(ctx, p, positions_host, tokens * sizeof(int32_t)));
+    check(ctx, nrs_sync(ctx));   // the caller's array may go away
+  }
+  const int32_t* pos = (const int32_t*)positions.get();
+  const float* table = norm.table ? norm.table->data : nullptr;
+  const int64_t wq = (int64_t)(heads_q * d), wk = (int64_t)(heads_k * d);
+  auto gamma_of = [](const NodeP& n) { return n ? n->data : nullptr; };
+  auto result = [&](const NodeP& x, const NodeP& gamma) {
+    std::vector<NodeP> parents{x};
+    for (const NodeP& n : {gamma, norm.table})
+      if (n) parents.push_back(n);
+    return make_result(ctx, x->shape, parents);
+  };
+  QueryKey out{result(q, norm.gamma_q), result(k, norm.gamma_k)};
+  check(ctx, nrs_qk_norm_rotary_fwd(ctx, q->data, wq, k->data, wk, gamma_of(norm.gamma_q), gamma_of(norm.gamma_k), table, pos, out.q->data, wq,
+                                    out.k->data, wk, (int)tokens, (int)seq, (int)heads_q, (int)heads_k, (int)d, rot, max_len, norm.interleaved ? 1 : 0,
+                                    norm.eps));
+  auto backward = [&](const NodeP& result, const NodeP& x, const NodeP& gamma, size_t heads) {
+    Node* self = result.get();
+    const bool inter = norm.interleaved;
+    const float eps = norm.eps;
+    const NodeP tab = norm.table;
+    result->backward_fn = [self, x, gamma, tab, positions, tokens, seq, heads, d, rot, max_len, inter, eps]() {
+      nrs_ctx* ctx = self->ctx;
+      if (!x->requires_grad && !(gamma && gamma->requires_grad)) return;
+      const float* g = grad_view(self);
+      const int64_t w = (int64_t)(heads * d);
+      GradSlot tx{nullptr, 0}, tg{nullptr, 0};
+      if (x->requires_grad) tx = grad_slot(x);
+      if (gamma && gamma->requires_grad) tg = grad_slot(gamma);
+      const size_t bytes = nrs_qk_norm_rotary_workspace((int)tokens, (int)heads, 0, (int)d);
+      void* ws = nullptr;
+      check(ctx, nrs_alloc(ctx, std::max<size_t>(16, bytes), 0, &ws));
+      const int st = nrs_qk_norm_rotary_bwd(ctx, g, w, nullptr, 0, x->data, w, nullptr, 0, gamma ? gamma->data : nullptr, nullptr, tab ? tab->data : nullptr,
+                                            (const int32_t*)positions.get(), tx.ptr, w, nullptr, 0, tg.ptr, nullptr, (int)tokens, (int)seq, (int)heads, 0,
+                                            (int)d, rot, max_len, inter ? 1 : 0, eps, tx.accumulate, tg.accumulate, ws, bytes);
+      nrs_free(ctx, ws);
+      check(ctx, st);
+    };
+  };
+  backward(out.q, q, norm.gamma_q, heads_q);
+  backward(out.k, k, norm.gamma_k, heads_k);
+  return out;
+}
+
 // Projections and attention core over operand planes (attention_planes.cu) as one node: x [tokens, d] -> [tokens, d], the
 // heads' results side by side.  One product makes Q, K and V, one sums the three shares of x's gradient, one makes the
 // three weight gradients.
@@ -348,12 +428,17 @@ NodeP MultiHeadAttention::forward_batch(const NodeP& x) const {
   if (!x || x->shape.size() != 3) fail(NRS_ERR_SHAPE, "cuda mha: input must be [batch, seq, d_model]");
   const size_t batch = x->shape[0], seq = x->shape[1], d = x->shape[2];
   if (d != d_model || num_heads == 0 || d_model % num_heads != 0) fail(NRS_ERR_SHAPE, "cuda mha: d_model / num_heads mismatch");
-  if (x->on_gpu() && planes_attention_applies(*this, x, batch, seq)) {
+  if (x->on_gpu() && !head_norm && planes_attention_applies(*this, x, batch, seq)) {
     NodeP flat = reshape(x, {batch * seq, d});
     return reshape(matmul(planes_attention(*this, flat, batch, seq), w_o), {batch, seq, d});
   }
   auto proj = [&](const NodeP& w) { return reshape(matmul(reshape(x, {batch * seq, d}), w), {batch, seq, d}); };
   NodeP q = proj(w_q), k = proj(w_k), v = proj(w_v);
+  if (head_norm) {
+    const QueryKey n = qk_norm_rotary(q, k, num_heads, num_heads, *head_norm);
+    q = n.q;
+    k = n.k;
+  }
   // The reference slices the heads out column by column, runs attention_batch per head and
   // concatenates (multihead.rs:94-107).  The same arithmetic in one pass: heads become extra
   // batch entries, attention_batch runs once over [batch*heads, seq, d_head].

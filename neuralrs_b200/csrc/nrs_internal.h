@@ -429,6 +429,18 @@ inline const NrsWeightPlanes* nrs_weight_planes_find(nrs_ctx* ctx, const void* w
                       cudaGetErrorString(e__));                                          \
   } while (0)
 
+// Makes the context's device the current one for a scope: its stream takes launches from there only.
+struct NrsDeviceGuard {
+  int was = -1;
+  explicit NrsDeviceGuard(const nrs_ctx* ctx) {
+    int now = -1;
+    if (cudaGetDevice(&now) == cudaSuccess && now != ctx->device && cudaSetDevice(ctx->device) == cudaSuccess) was = now;
+  }
+  ~NrsDeviceGuard() { if (was >= 0) (void)cudaSetDevice(was); }
+  NrsDeviceGuard(const NrsDeviceGuard&) = delete;
+  NrsDeviceGuard& operator=(const NrsDeviceGuard&) = delete;
+};
+
 // cudaFuncAttributeMaxDynamicSharedMemorySize belongs to a (kernel, device) pair, and one process may hold
 // contexts on several devices.  Each launcher keeps one NrsSmemAttr per kernel instantiation: the largest
 // value already set on every device ordinal.

@@ -390,7 +390,8 @@ class nn:
 
     @staticmethod
     def dropout(x: Node, p: float, training: bool, mask: Node | None = None) -> Node:
-        """src/cuda/nn/dropout.rs:31-84.  mask=None draws the mask on the device (context seed and counter)."""
+        """src/cuda/nn/dropout.rs:31-84.  mask=None draws the mask on the device (context seed and counter) in each pass and
+        stores none."""
         h = VP()
         return _out(x.ctx, x.ctx._l.nrs_op_dropout(x.h, C.c_float(p), int(training), mask.h if mask else None, C.byref(h)), h)
 
@@ -399,6 +400,12 @@ class nn:
         """src/cuda/nn/dropout2d.rs: one mask value per (sample, channel) plane."""
         h = VP()
         return _out(x.ctx, x.ctx._l.nrs_op_dropout2d(x.h, C.c_float(p), int(training), mask.h if mask else None, C.byref(h)), h)
+
+    @staticmethod
+    def dropout_add(x: Node, residual: Node, p: float, training: bool) -> Node:
+        """residual + dropout(x) in one pass; no mask is stored (no reference counterpart)."""
+        h = VP()
+        return _out(x.ctx, x.ctx._l.nrs_op_dropout_add(x.h, residual.h, C.c_float(p), int(training), C.byref(h)), h)
 
     @staticmethod
     def linear_act(x: Node, w: Node, b: Node, act: int) -> Node:
@@ -453,18 +460,58 @@ class nn:
             h = VP()
             return _out(x.ctx, x.ctx._l.nrs_op_positional(x.h, self.table.h, C.byref(h)), h)
 
-    class MultiHeadAttention:
-        """src/cuda/nn/multihead.rs:20-85 (weights [d,d], no biases)."""
+    class RotaryEmbedding:
+        """cos and sin of every position's angles, [max_len, rot_dim], made once and kept on the device (no reference
+        counterpart)."""
 
-        def __init__(self, w_q, w_k, w_v, w_o, d_model: int, num_heads: int, causal: bool = False):
+        def __init__(self, rot_dim: int, max_len: int, base: float = 10000.0, ctx: Context | None = None):
+            ctx = ctx or default_context()
+            h = VP()
+            check(ctx.h, ctx._l.nrs_rotary_new(ctx.h, int(rot_dim), int(max_len), C.c_float(base), C.byref(h)))
+            self.table = Node(h, ctx)
+            self.rot_dim, self.max_len = rot_dim, max_len
+
+    class HeadNorm:
+        """RMS norm of every query and key head with the rotation of its position, in one pass (no reference counterpart).
+        gamma_q, gamma_k: [d_head] or None; rotary: an nn.RotaryEmbedding or None."""
+
+        def __init__(self, gamma_q: Node | None, gamma_k: Node | None, rotary=None, interleaved: bool = False, eps: float = 1e-6):
+            self.gamma_q, self.gamma_k, self.rotary, self.interleaved, self.eps = gamma_q, gamma_k, rotary, interleaved, eps
+
+        def parameters(self):
+            return [g for g in (self.gamma_q, self.gamma_k) if g is not None]
+
+        def _handles(self):
+            return [n.h if n is not None else None for n in (self.gamma_q, self.gamma_k, self.rotary.table if self.rotary else None)]
+
+        def forward(self, q: Node, k: Node, heads_q: int, heads_k: int, positions=None) -> tuple[Node, Node]:
+            """q [.., seq, heads_q * d], k [.., seq, heads_k * d]; positions: one per token, None for the place in the sequence."""
+            hq, hk = VP(), VP()
+            pos = None if positions is None else np.ascontiguousarray(positions, dtype=np.int32).reshape(-1)
+            if pos is not None and pos.size * q.shape[-1] != len(q):
+                raise ValueError("one position per token is needed")
+            check(q.ctx.h, q.ctx._l.nrs_op_qk_norm_rotary(q.h, k.h, *self._handles(), _ptr(pos) if pos is not None else None, int(heads_q),
+                                                          int(heads_k), int(self.interleaved), C.c_float(self.eps), C.byref(hq), C.byref(hk)))
+            return Node(hq, q.ctx), Node(hk, q.ctx)
+
+    class MultiHeadAttention:
+        """src/cuda/nn/multihead.rs:20-85 (weights [d,d], no biases).  head_norm (an nn.HeadNorm, an extension): norms and
+        rotations of the projected queries and keys."""
+
+        def __init__(self, w_q, w_k, w_v, w_o, d_model: int, num_heads: int, causal: bool = False, head_norm=None):
             self.w_q, self.w_k, self.w_v, self.w_o = w_q, w_k, w_v, w_o
-            self.d_model, self.num_heads, self.causal = d_model, num_heads, causal
+            self.d_model, self.num_heads, self.causal, self.head_norm = d_model, num_heads, causal, head_norm
 
         def parameters(self):
             return [self.w_q, self.w_k, self.w_v, self.w_o]
 
         def forward_batch(self, x: Node) -> Node:
             h = VP()
+            if self.head_norm is not None:
+                n = self.head_norm
+                return _out(x.ctx, x.ctx._l.nrs_op_mha_rotary(x.h, self.w_q.h, self.w_k.h, self.w_v.h, self.w_o.h, *n._handles(),
+                                                              int(self.num_heads), int(n.interleaved), C.c_float(n.eps),
+                                                              int(self.causal), C.byref(h)), h)
             return _out(x.ctx, x.ctx._l.nrs_op_mha(x.h, self.w_q.h, self.w_k.h, self.w_v.h, self.w_o.h,
                                                   int(self.num_heads), int(self.causal), C.byref(h)), h)
 
@@ -480,6 +527,8 @@ class nn:
                                             self.ff1.weights, self.ff1.bias, self.ff2.weights, self.ff2.bias]
 
         def _run(self, x: Node, final_norm: bool) -> Node:
+            if self.mha.head_norm is not None:
+                raise ValueError("TransformerBlock runs attention without head norms; compose the block from its parts")
             h = VP()
             return _out(x.ctx, x.ctx._l.nrs_op_transformer_block(
                 x.h, _handles(self.parameters()), int(self.mha.num_heads), C.c_float(self.norm1.eps), int(self.act),

@@ -49,6 +49,7 @@ pub const NRS_MATH_FP32: i32 = 2;
 pub const NRS_ACT_NONE: i32 = 0;
 pub const NRS_ACT_RELU: i32 = 1;
 pub const NRS_ACT_GELU: i32 = 2;
+pub const NRS_ACT_SILU: i32 = 3;
 
 extern "C" {
 '''
