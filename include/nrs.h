@@ -379,6 +379,17 @@ int nrs_embedding_pos_fwd(nrs_ctx* ctx, const float* weight, const int32_t* idx,
                           int tokens, int seq, int dim, int vocab);
 int nrs_embedding_bwd(nrs_ctx* ctx, const float* g, const int32_t* idx, float* dweight, int tokens, int dim,
                       int vocab, int accumulate);
+/* Lookup with a scale (no reference counterpart; embed_forward above has none): out[t,:] = scale * weight[idx[t],:]
+ * (+ pos_table[t % seq,:] when given), ids checked as there.  And the gradient of it by sorted tokens: dweight[v,:] (+)=
+ * scale * the sum of g[t,:] over the tokens with idx[t] == v, in one fixed order (deterministic).  An id outside the
+ * vocabulary contributes nothing.  accumulate == 0 writes every row of dweight, zeros where no token is.  The workspace, at
+ * least nrs_embedding_sorted_workspace bytes, is used by this call alone: calls that may run at the same time (two
+ * captured graphs) bring one each.  tokens up to 2^30. */
+int nrs_embedding_scaled_fwd(nrs_ctx* ctx, const float* weight, const int32_t* idx, const float* pos_table, float* out,
+                             int tokens, int seq, int dim, int vocab, float scale);
+size_t nrs_embedding_sorted_workspace(int tokens, int dim, int vocab);
+int nrs_embedding_sorted_bwd(nrs_ctx* ctx, const float* g, const int32_t* idx, float* dweight, int tokens, int dim,
+                             int vocab, float scale, int accumulate, void* workspace, size_t workspace_bytes);
 /* Causal mask over [batch, s, s] attention scores.  No reference counterpart (the
  * reference has no mask).  backward == 0: y = (j > i) ? -1e30 : x;
  * backward != 0: y (+)= (j > i) ? 0 : x. */

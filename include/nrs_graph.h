@@ -112,6 +112,9 @@ int nrs_op_conv2d_act(nrs_node* input, nrs_node* weight, nrs_node* bias, int64_t
  * is a HOST array of token ids, checked against the weight's row count. */
 int nrs_op_embedding(nrs_node* weight, const int32_t* indices_host, int64_t count, nrs_node** out);
 int nrs_op_embedding_batch(nrs_node* weight, const int32_t* indices_host, int64_t batch, int64_t seq, nrs_node** out);
+/* The batched form with the rows times `scale` (not 0; sqrt(dim) in many token models) and the weight's gradient from
+ * sorted tokens (nrs_embedding_sorted_bwd).  No reference counterpart. */
+int nrs_op_embedding_scaled(nrs_node* weight, const int32_t* indices_host, int64_t batch, int64_t seq, float scale, nrs_node** out);
 /* PositionalEncoding::new(d_model, max_len): the resident sinusoidal table, and
  * forward(x) = x + table[:seq] for x [seq, d] or [batch, seq, d]. */
 int nrs_positional_new(nrs_ctx* ctx, int64_t d_model, int64_t max_len, nrs_node** table_out);
@@ -191,7 +194,8 @@ enum nrs_layer_kind {
   /* Token models.  An embedding layer must be the first layer: the model then reads int32 token ids
    * [batch, seq] (in_shape = {seq}) through the *_tokens entry points, activations are [batch, seq, d],
    * a linear layer acts on every position, and the loss runs over batch*seq rows. */
-  NRS_LAYER_EMBEDDING = 9, /* a=vocab b=d_model c=max_len: Embedding::forward_batch (src/nn/embedding.rs:60-113)
+  NRS_LAYER_EMBEDDING = 9, /* a=vocab b=d_model c=max_len d=flags (bit 0: rows times sqrt(d_model), gradient by sorted
+                              tokens, as nrs_op_embedding_scaled): Embedding::forward_batch (src/nn/embedding.rs:60-113)
                               followed, when c > 0, by PositionalEncoding::new(d_model, max_len).forward
                               (src/cuda/nn/positional.rs:18-44), both in one gather kernel               */
   NRS_LAYER_TRANSFORMER_BLOCK = 10, /* a=d_model b=num_heads c=d_ff d=activation (NRS_ACT_RELU as

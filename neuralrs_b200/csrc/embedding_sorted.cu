@@ -1,0 +1,433 @@
+// Embedding lookup with a scale, and the table's gradient from tokens sorted by their ids.
+//
+//   out[t, :] = scale * weight[id_t, :] (+ pos[t % seq, :])
+//   dweight[v, :] (+)= scale * sum over the tokens with id_t = v, in the order of t, of g[t, :]
+//
+// Lookup as in the reference's embed_forward (src/cuda/nn/embedding.rs:13-21), which has no scale.  Its gradient adds every
+// token's row with atomics (:23-30); the form in transformer.cu gives every vocabulary row a block that looks through all
+// tokens, vocab * tokens comparisons.  Here two launches do tokens' work alone:
+//
+//   sort   every block owns a range of the vocabulary.  It looks through all ids once (they stay in L2), counts those below
+//          its range, which is where its own tokens start in the sorted order, and lists its own in the order of t; a
+//          stable counting sort of the list by id then needs no other block.  It writes the sorted (id, token) pairs and
+//          where each row's run starts, and zeroes the rows of the gradient that no token has.
+//   sum    the sorted tokens are cut into equal pieces, so a token that makes up a tenth of the text costs no block more
+//          than its share.  A run inside one piece goes straight to its row; one that crosses pieces leaves partial sums,
+//          and the last of its blocks to finish adds them up, in order.
+//
+// Deterministic: every sum has one order, whatever the blocks' timing.  Bound by memory: g read once, dweight written once.
+#include <algorithm>
+
+#include "nrs_internal.h"
+
+namespace {
+
+constexpr int kErrBadIndex = 5;
+
+// ------------------------------------------------------------------------------------------------ lookup
+
+// One vector (VEC: 16 bytes) of a row per thread and step, four under way together.
+template <bool VEC>
+__global__ void __launch_bounds__(256)
+embed_scaled_kernel(const float* __restrict__ w, const int32_t* __restrict__ idx, const float* __restrict__ pos, float* __restrict__ out, size_t total,
+                    int width /*vectors of a row*/, int seq, int vocab, float scale, int* err) {
+  NRS_PDL_PROLOGUE();
+  constexpr int kDeep = 4;
+  const size_t stride = (size_t)gridDim.x * blockDim.x;
+  for (size_t i0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i0 < total; i0 += kDeep * stride) {
+    float4 v[kDeep], p[kDeep];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const size_t i = i0 + k * stride;
+      v[k] = p[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i >= total) continue;
+      const size_t t = (i >> 32) ? i / (size_t)width : (size_t)((uint32_t)i / (uint32_t)width);
+      const int c = (int)(i - t * width), row = idx[t];
+      if (row >= 0 && row < vocab) {
+        const size_t at = (size_t)row * width + c;
+        if (VEC) v[k] = reinterpret_cast<const float4*>(w)[at];
+        else v[k].x = w[at];
+      } else if (c == 0) {
+        atomicExch(err, kErrBadIndex);
+      }
+      if (pos) {
+        const size_t at = (size_t)((uint32_t)t % (uint32_t)seq) * width + c;
+        if (VEC) p[k] = reinterpret_cast<const float4*>(pos)[at];
+        else p[k].x = pos[at];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const size_t i = i0 + k * stride;
+      if (i >= total) continue;
+      if (VEC) reinterpret_cast<float4*>(out)[i] = make_float4(fmaf(scale, v[k].x, p[k].x), fmaf(scale, v[k].y, p[k].y), fmaf(scale, v[k].z, p[k].z),
+                                                               fmaf(scale, v[k].w, p[k].w));
+      else out[i] = fmaf(scale, v[k].x, p[k].x);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sort
+
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kTile = 4 * kSortThreads;   // tokens of a step: four neighbouring ids a thread
+constexpr int kMaxRange = 8192;           // most vocabulary rows of a block
+constexpr int kSumWarps = 8;              // of a block that sums
+constexpr int kSlab = 128;                // its columns
+constexpr int kFillBlocks = 592;          // four for each of 148 SMs: fewer and pieces are made smaller
+
+struct Plan {
+  int tokens, dim, vocab, range;      // range: vocabulary rows of a sorting block
+  int slabs, per_warp, pieces;        // sum: slabs of a row, tokens of a warp, pieces of the sorted tokens
+  __host__ __device__ int piece() const { return kSumWarps * per_warp; }
+};
+Plan plan_of(int tokens, int dim, int vocab, int sm_count) {
+  Plan p{tokens, dim, vocab, 0, (dim + kSlab - 1) / kSlab, 32, 0};
+  p.range = std::min(kMaxRange, (vocab + sm_count - 1) / sm_count);
+  while (p.per_warp > 4 && (long)((tokens + p.piece() - 1) / p.piece()) * p.slabs < kFillBlocks) p.per_warp /= 2;
+  p.pieces = (tokens + p.piece() - 1) / p.piece();
+  return p;
+}
+struct Work {            // in the caller's workspace, in this order
+  int2* sorted;          // [tokens] (id, token)
+  float* partial;        // [pieces][2][dim] sums of a piece's tokens whose run came from before it, and of those whose run goes on
+  unsigned* tickets;     // [pieces][slabs] how many pieces of the run that starts in a piece are done
+  int* start;            // [vocab + 1] first sorted token of each row
+};
+size_t work_of(const Plan& p, void* base, Work* w) {
+  uint8_t* at = (uint8_t*)base;
+  size_t used = 0;
+  auto take = [&](size_t bytes) {
+    void* q = at + used;
+    used += (bytes + 255) / 256 * 256;
+    return q;
+  };
+  Work x;
+  x.sorted = (int2*)take(sizeof(int2) * p.tokens);
+  x.partial = (float*)take(sizeof(float) * 2 * p.pieces * p.dim);
+  x.tickets = (unsigned*)take(sizeof(unsigned) * p.pieces * p.slabs);
+  x.start = (int*)take(sizeof(int) * ((size_t)p.vocab + 1));
+  if (w) *w = x;
+  return used;
+}
+
+__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
+__device__ __forceinline__ int warp_scan(int v, int lane) {   // inclusive
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+__device__ __forceinline__ void four_ids(const int32_t* idx, int t, int tokens, bool quads, int (&id)[4]) {
+  if (quads && t + 4 <= tokens) {
+    const int4 q = *reinterpret_cast<const int4*>(idx + t);
+    id[0] = q.x; id[1] = q.y; id[2] = q.z; id[3] = q.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) id[k] = t + k < tokens ? idx[t + k] : -1;
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads, 1)
+embed_sort_kernel(const int32_t* __restrict__ idx, const Plan p, const Work w, float* __restrict__ dw /*null: rows without tokens stay*/, bool vec) {
+  NRS_PDL_PROLOGUE();
+  extern __shared__ int smem[];
+  int2* list = reinterpret_cast<int2*>(smem);      // [kTile] a step's own tokens, in order
+  int* next = smem + 2 * kTile;                    // [range] tokens of each row, then where its next one goes
+  __shared__ int s_warp[2][kSortWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lo = blockIdx.x * p.range, hi = min(p.vocab, lo + p.range), rows = hi - lo;
+  const bool quads = (reinterpret_cast<uintptr_t>(idx) & 15) == 0;
+  for (int i = tid; i < rows; i += kSortThreads) next[i] = 0;
+  for (long i = (long)blockIdx.x * kSortThreads + tid; i < (long)p.pieces * p.slabs; i += (long)gridDim.x * kSortThreads) w.tickets[i] = 0;
+  __syncthreads();
+
+  // How many tokens each row has, and how many lie below the range.  (Ids outside the vocabulary are nobody's.)
+  int below = 0;
+  for (int t0 = 0; t0 < p.tokens; t0 += kTile) {
+    int id[4];
+    four_ids(idx, t0 + 4 * tid, p.tokens, quads, id);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      below += id[k] >= 0 && id[k] < lo;
+      if (id[k] >= lo && id[k] < hi) atomicAdd(&next[id[k] - lo], 1);
+    }
+  }
+  below = warp_sum(below);
+  if (lane == 0) s_warp[0][warp] = below;
+  __syncthreads();
+  const int first = warp_sum(s_warp[0][lane]);     // where the range starts in the sorted order
+
+  // Counts to starts: a stretch of rows a thread.
+  const int each = (rows + kSortThreads - 1) / kSortThreads, r0 = min(rows, tid * each), r1 = min(rows, r0 + each);
+  int sum = 0;
+  for (int r = r0; r < r1; ++r) sum += next[r];
+  const int incl = warp_scan(sum, lane);
+  if (lane == 31) s_warp[1][warp] = incl;
+  __syncthreads();
+  int run = first + warp_sum(lane < warp ? s_warp[1][lane] : 0) + incl - sum;
+  for (int r = r0; r < r1; ++r) {
+    const int c = next[r];
+    next[r] = w.start[lo + r] = run;
+    run += c;
+  }
+  if (hi == p.vocab && r1 == rows && (r0 < rows || tid == 0)) w.start[p.vocab] = run;
+  __syncthreads();
+  const int end = first + warp_sum(s_warp[1][lane]);
+
+  // Each own token behind those of its id that came before it.
+  if (end > first) {
+    for (int t0 = 0, step = 0; t0 < p.tokens; t0 += kTile, ++step) {
+      const int t = t0 + 4 * tid;
+      int id[4], mine = 0;
+      four_ids(idx, t, p.tokens, quads, id);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mine += id[k] >= lo && id[k] < hi;
+      const int before = warp_scan(mine, lane);
+      __syncthreads();                             // the step before has read its counts and its list
+      if (lane == 31) s_warp[0][warp] = before;
+      __syncthreads();
+      const int h = s_warp[0][lane], found = warp_sum(h);
+      int at = warp_sum(lane < warp ? h : 0) + before - mine;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (id[k] >= lo && id[k] < hi) list[at++] = make_int2(id[k] - lo, t + k);
+      __syncthreads();
+      if (warp == 0) {
+        for (int i0 = 0; i0 < found; i0 += 32) {
+          const bool on = i0 + lane < found;
+          const int2 e = on ? list[i0 + lane] : make_int2(-1, 0);
+          const unsigned same = __match_any_sync(0xffffffffu, e.x);
+          const int rank = __popc(same & ((1u << lane) - 1u)), to = on ? next[e.x] + rank : 0;
+          __syncwarp();
+          if (on) {
+            w.sorted[to] = make_int2(e.x + lo, e.y);
+            if (rank == 0) next[e.x] = to + __popc(same);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  if (!dw) return;
+  __syncthreads();
+  // Rows without a token: `next` now holds where each ends.
+  for (int r = warp; r < rows; r += kSortWarps) {
+    if (next[r] != (r ? next[r - 1] : first)) continue;
+    float* row = dw + (size_t)(lo + r) * p.dim;
+    if (vec)
+      for (int c = lane; c < p.dim / 4; c += 32) reinterpret_cast<float4*>(row)[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    else
+      for (int c = lane; c < p.dim; c += 32) row[c] = 0.0f;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sum
+
+// A lane's four columns of a slab: neighbours (VEC), or 32 apart.
+template <bool VEC>
+struct Cols {
+  int c0, dim;
+  __device__ __forceinline__ void load(float (&v)[4], const float* row) const {
+    if (VEC) {
+      const float4 q = c0 < dim ? *reinterpret_cast<const float4*>(row + c0) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = c0 + 32 * j < dim ? row[c0 + 32 * j] : 0.0f;
+    }
+  }
+  __device__ __forceinline__ void store(const float (&v)[4], float* row) const {
+    if (VEC) {
+      if (c0 < dim) *reinterpret_cast<float4*>(row + c0) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c0 + 32 * j < dim) row[c0 + 32 * j] = v[j];
+    }
+  }
+};
+
+template <bool VEC>
+__global__ void __launch_bounds__(kSumWarps * 32)
+embed_sum_kernel(const float* __restrict__ g, const Plan p, const Work w, float* dw, float scale, int accumulate) {
+  NRS_PDL_PROLOGUE();
+  __shared__ float4 s_head[kSumWarps][32], s_tail[kSumWarps][32];
+  __shared__ int s_flags[kSumWarps];               // 1: has a sum for a run from before; 2: for one that goes on; 4: both are one run
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int piece = blockIdx.x / p.slabs, slab = blockIdx.x - piece * p.slabs;
+  const Cols<VEC> cols{slab * kSlab + (VEC ? 4 * lane : lane), p.dim};
+  const int valid = w.start[p.vocab];              // tokens with an id of the vocabulary
+  const int base = piece * p.piece() + warp * p.per_warp, n = min(p.per_warp, valid - base);
+
+  auto finish = [&](int id, const float (&a)[4]) {   // a row's sum is complete
+    float* row = dw + (size_t)id * p.dim;
+    float r[4];
+    if (accumulate) {
+      cols.load(r, row);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = fmaf(scale, a[j], r[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = scale * a[j];
+    }
+    cols.store(r, row);
+  };
+
+  int flags = 0, id_first = -1, id_last = -1;
+  if (n > 0) {
+    const int2 e = lane < n ? w.sorted[base + lane] : make_int2(-1, 0);
+    const int edge = lane == 0 ? (base > 0 ? w.sorted[base - 1].x : -1) : lane == 1 ? (base + n < valid ? w.sorted[base + n].x : -1) : 0;
+    id_first = __shfl_sync(0xffffffffu, e.x, 0);
+    id_last = __shfl_sync(0xffffffffu, e.x, n - 1);
+    const bool from_before = __shfl_sync(0xffffffffu, edge, 0) == id_first, goes_on = __shfl_sync(0xffffffffu, edge, 1) == id_last;
+    float acc[4] = {};
+    int id = id_first;
+    bool first_run = true;
+    constexpr int kDeep = 8;
+    for (int i0 = 0; i0 < n; i0 += kDeep) {
+      float v[kDeep][4];
+#pragma unroll
+      for (int k = 0; k < kDeep; ++k) {
+        if (i0 + k >= n) break;
+        cols.load(v[k], g + (size_t)__shfl_sync(0xffffffffu, e.y, i0 + k) * p.dim);
+      }
+#pragma unroll
+      for (int k = 0; k < kDeep; ++k) {
+        if (i0 + k >= n) break;
+        const int now = __shfl_sync(0xffffffffu, e.x, i0 + k);
+        if (now != id) {
+          if (first_run && from_before) {
+            s_head[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            flags |= 1;
+          } else {
+            finish(id, acc);
+          }
+          first_run = false;
+          id = now;
+          acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += v[k][j];
+      }
+    }
+    const bool head = first_run && from_before;
+    if (head) {
+      s_head[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      flags |= goes_on ? 5 : 1;
+    } else if (goes_on) {
+      s_tail[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      flags |= 2;
+    } else {
+      finish(id, acc);
+    }
+  }
+  if (lane == 0) s_flags[warp] = flags;
+  __syncthreads();
+
+  // The sums of one run that lie in several warps: added up by the warp where it starts, or (a run from an earlier piece)
+  // the first.  A warp may have two such runs.
+  auto chain = [&](bool incoming) {
+    const int id = incoming ? id_first : id_last;
+    const float4 q = incoming ? s_head[warp][lane] : s_tail[warp][lane];
+    float a[4] = {q.x, q.y, q.z, q.w};
+    bool on = incoming ? (flags & 4) != 0 : true;  // the run goes on behind this warp
+    for (int k = warp + 1; on && k < kSumWarps; ++k) {
+      const float4 o = s_head[k][lane];
+      a[0] += o.x; a[1] += o.y; a[2] += o.z; a[3] += o.w;
+      on = (s_flags[k] & 4) != 0;
+    }
+    if (!incoming && !on) {
+      finish(id, a);
+      return;
+    }
+    // The run crosses pieces: the last of them to get here adds their sums up, in order.
+    const int from = w.start[id] / p.piece(), to = (w.start[id + 1] - 1) / p.piece();
+    cols.store(a, w.partial + ((size_t)piece * 2 + (incoming ? 0 : 1)) * p.dim);
+    __threadfence();
+    __syncwarp();
+    unsigned done = 0;
+    if (lane == 0) done = atomicAdd(&w.tickets[(size_t)from * p.slabs + slab], 1u);
+    if (__shfl_sync(0xffffffffu, done, 0) != (unsigned)(to - from)) return;
+    __threadfence();
+    cols.load(a, w.partial + ((size_t)from * 2 + 1) * p.dim);
+    constexpr int kDeep = 8;
+    for (int k0 = from + 1; k0 <= to; k0 += kDeep) {
+      float v[kDeep][4];
+#pragma unroll
+      for (int k = 0; k < kDeep; ++k) {
+        if (k0 + k > to) break;
+        cols.load(v[k], w.partial + (size_t)(k0 + k) * 2 * p.dim);
+      }
+#pragma unroll
+      for (int k = 0; k < kDeep; ++k) {
+        if (k0 + k > to) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] += v[k][j];
+      }
+    }
+    finish(id, a);
+  };
+  if (warp == 0 && (flags & 1)) chain(true);
+  if (flags & 2) chain(false);
+}
+
+}  // namespace
+
+extern "C" {
+
+int nrs_embedding_scaled_fwd(nrs_ctx* ctx, const float* weight, const int32_t* idx, const float* pos_table, float* out, int tokens, int seq, int dim,
+                             int vocab, float scale) {
+  NRS_REQUIRE_CTX(ctx);
+  NRS_REQUIRE(ctx, tokens >= 0 && dim > 0 && vocab > 0, NRS_ERR_SHAPE, "%s: bad shape [%d,%d], vocabulary %d", __func__, tokens, dim, vocab);
+  NRS_REQUIRE(ctx, !pos_table || seq > 0, NRS_ERR_SHAPE, "%s: sequence length must be positive", __func__);
+  if (tokens == 0) return NRS_OK;
+  NRS_REQUIRE(ctx, weight && idx && out, NRS_ERR_ARG, "%s: null tensor", __func__);
+  NrsDeviceGuard on(ctx);
+  int* err = nullptr;
+  const int st = nrs_err_flag(ctx, &err);
+  if (st != NRS_OK) return st;
+  const bool vec = dim % 4 == 0 && (((uintptr_t)weight | (uintptr_t)out | (uintptr_t)pos_table) & 15) == 0;
+  const int width = vec ? dim / 4 : dim;
+  const size_t total = (size_t)tokens * width, want = (total + 255) / 256, cap = (size_t)ctx->sm_count * 16;
+  const unsigned blocks = (unsigned)(want < cap ? want : cap);
+  if (vec) NRS_PDL_LAUNCH(embed_scaled_kernel<true>, blocks, 256, 0, ctx->stream, weight, idx, pos_table, out, total, width, seq > 0 ? seq : 1, vocab, scale, err);
+  else NRS_PDL_LAUNCH(embed_scaled_kernel<false>, blocks, 256, 0, ctx->stream, weight, idx, pos_table, out, total, width, seq > 0 ? seq : 1, vocab, scale, err);
+  NRS_LAUNCHED(ctx);
+  return NRS_OK;
+}
+
+size_t nrs_embedding_sorted_workspace(int tokens, int dim, int vocab) {
+  if (tokens < 0 || dim <= 0 || vocab <= 0) return 0;
+  return work_of(plan_of(tokens, dim, vocab, 1), nullptr, nullptr);
+}
+
+int nrs_embedding_sorted_bwd(nrs_ctx* ctx, const float* g, const int32_t* idx, float* dweight, int tokens, int dim, int vocab, float scale, int accumulate,
+                             void* workspace, size_t workspace_bytes) {
+  NRS_REQUIRE_CTX(ctx);
+  NRS_REQUIRE(ctx, tokens >= 0 && dim > 0 && vocab > 0 && tokens <= (1 << 30), NRS_ERR_SHAPE, "%s: bad shape [%d,%d], vocabulary %d", __func__, tokens, dim, vocab);
+  if (tokens == 0 && accumulate) return NRS_OK;
+  NRS_REQUIRE(ctx, dweight && (tokens == 0 || (g && idx)), NRS_ERR_ARG, "%s: null tensor", __func__);
+  const Plan p = plan_of(tokens, dim, vocab, ctx->sm_count);
+  Work w{};
+  const size_t need = work_of(p, workspace, &w);
+  NRS_REQUIRE(ctx, workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, NRS_ERR_ARG,
+              "%s: needs a workspace of %zu bytes on a 16-byte boundary", __func__, need);
+  NRS_REQUIRE(ctx, (long)p.pieces * p.slabs <= 0x7fffffffL, NRS_ERR_SHAPE, "%s: %d tokens of %d features are too many for one call", __func__, tokens, dim);
+  NrsDeviceGuard on(ctx);
+  const bool vec = dim % 4 == 0 && (((uintptr_t)g | (uintptr_t)dweight) & 15) == 0;
+  const size_t smem = sizeof(int2) * kTile + sizeof(int) * p.range;
+  static NrsSmemAttr attr;
+  NRS_ENSURE_SMEM(ctx, attr, embed_sort_kernel, smem);
+  NRS_PDL_LAUNCH(embed_sort_kernel, (vocab + p.range - 1) / p.range, kSortThreads, smem, ctx->stream, idx, p, w, accumulate ? nullptr : dweight, vec);
+  NRS_LAUNCHED(ctx);
+  if (tokens == 0) return NRS_OK;
+  if (vec) NRS_PDL_LAUNCH(embed_sum_kernel<true>, p.pieces * p.slabs, kSumWarps * 32, 0, ctx->stream, g, p, w, dweight, scale, accumulate != 0);
+  else NRS_PDL_LAUNCH(embed_sum_kernel<false>, p.pieces * p.slabs, kSumWarps * 32, 0, ctx->stream, g, p, w, dweight, scale, accumulate != 0);
+  NRS_LAUNCHED(ctx);
+  return NRS_OK;
+}
+
+}  // extern "C"

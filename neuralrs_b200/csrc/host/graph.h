@@ -235,6 +235,7 @@ struct LayerNorm {                    // normalization.rs (struct form of layern
 struct Embedding {                    // embedding.rs:41-100
   NodeP weight;
   size_t vocab_size = 0, embedding_dim = 0;
+  float scale = 0.0f;                 // not 0: rows come times this factor, and the gradient by sorted tokens (extension)
   // indices: `count` token ids; result is [count, dim] (forward) or [batch, seq, dim] (forward_batch,
   // which the reference has on the CPU only: src/nn/embedding.rs:60-113).
   NodeP forward(const int32_t* indices, size_t count) const;

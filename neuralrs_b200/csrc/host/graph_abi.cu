@@ -320,6 +320,17 @@ int nrs_op_embedding_batch(nrs_node* weight, const int32_t* indices_host, int64_
   });
 }
 
+int nrs_op_embedding_scaled(nrs_node* weight, const int32_t* indices_host, int64_t batch, int64_t seq, float scale, nrs_node** out) {
+  NODE_OK(weight);
+  if (batch < 0 || seq < 0 || batch * seq > 2147483647 || weight->p->shape.size() != 2)
+    return nrs_fail(ctx_of(weight), NRS_ERR_SHAPE, "embedding: bad shape");
+  if (!(scale != 0.0f)) return nrs_fail(ctx_of(weight), NRS_ERR_ARG, "embedding: the scale must not be 0");
+  return wrap(ctx_of(weight), out, [&] {
+    nrs::cuda::Embedding e{weight->p, weight->p->shape[0], weight->p->shape[1], scale};
+    return e.forward_batch(indices_host, (size_t)batch, (size_t)seq);
+  });
+}
+
 int nrs_positional_new(nrs_ctx* ctx, int64_t d_model, int64_t max_len, nrs_node** table_out) {
   NRS_REQUIRE_CTX(ctx);
   NRS_REQUIRE(ctx, d_model > 0 && max_len > 0, NRS_ERR_SHAPE, "nrs_positional_new: non-positive size");

@@ -10,6 +10,7 @@
 //
 // The gradient exchange itself lives in dp.cu (DpGroup).
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <unordered_set>
 
@@ -262,6 +263,7 @@ NodeP forward(nrs_trainer* t, const NodeP& x, const int32_t* ids_dev, size_t bat
         e.weight = t->params[pi];
         e.vocab_size = (size_t)l.a;
         e.embedding_dim = (size_t)l.b;
+        if (l.d & 1) e.scale = std::sqrt((float)l.b);
         h = e.forward_resident(ids_dev, batch, t->in_shape[0], t->pos_table);
         pi += 1;
         break;

@@ -90,10 +90,27 @@ static NodeP embed_resident(const Embedding& e, const int32_t* idx_dev, size_t c
   nrs_ctx* ctx = e.weight->ctx;
   const int dim = (int)e.embedding_dim, vocab = (int)e.vocab_size;
   NodeP out = make_result(ctx, out_shape, {e.weight});
-  check(ctx, nrs_embedding_pos_fwd(ctx, e.weight->data, idx_dev, pos_table ? pos_table->data : nullptr, out->data, (int)count,
-                                   (int)seq, dim, vocab));
   Node* self = out.get();
   const NodeP w = e.weight;
+  if (e.scale != 0.0f) {
+    const float scale = e.scale;
+    check(ctx, nrs_embedding_scaled_fwd(ctx, w->data, idx_dev, pos_table ? pos_table->data : nullptr, out->data, (int)count, (int)seq, dim, vocab, scale));
+    out->backward_fn = [self, w, idx_dev, count, dim, vocab, scale]() {
+      if (!w->requires_grad) return;
+      nrs_ctx* ctx = self->ctx;
+      const float* g = grad_view(self);
+      GradSlot t = grad_slot(w);
+      const size_t bytes = nrs_embedding_sorted_workspace((int)count, dim, vocab);
+      void* ws = nullptr;
+      check(ctx, nrs_alloc(ctx, std::max<size_t>(16, bytes), 0, &ws));
+      const int st = nrs_embedding_sorted_bwd(ctx, g, idx_dev, t.ptr, (int)count, dim, vocab, scale, t.accumulate, ws, bytes);
+      nrs_free(ctx, ws);
+      check(ctx, st);
+    };
+    return out;
+  }
+  check(ctx, nrs_embedding_pos_fwd(ctx, e.weight->data, idx_dev, pos_table ? pos_table->data : nullptr, out->data, (int)count,
+                                   (int)seq, dim, vocab));
   out->backward_fn = [self, w, idx_dev, count, dim, vocab]() {
     if (!w->requires_grad) return;
     const float* g = grad_view(self);

@@ -428,13 +428,16 @@ class nn:
             return nn.layernorm(x, self.gamma, self.beta, self.eps)
 
     class Embedding:
-        """src/cuda/nn/embedding.rs:41-100; forward_batch mirrors src/nn/embedding.rs:60-113."""
+        """src/cuda/nn/embedding.rs:41-100; forward_batch mirrors src/nn/embedding.rs:60-113.  scale (an extension): rows come
+        times this factor, and the table's gradient is made from sorted tokens."""
 
-        def __init__(self, weight: Node, vocab_size: int, embedding_dim: int):
-            self.weight, self.vocab_size, self.embedding_dim = weight, vocab_size, embedding_dim
+        def __init__(self, weight: Node, vocab_size: int, embedding_dim: int, scale: float | None = None):
+            self.weight, self.vocab_size, self.embedding_dim, self.scale = weight, vocab_size, embedding_dim, scale
 
         def forward(self, indices) -> Node:
             idx = np.ascontiguousarray(indices, dtype=np.int32).reshape(-1)
+            if self.scale is not None:
+                return graph.reshape(self.forward_batch(idx[None]), [idx.size, self.embedding_dim])
             h = VP()
             l = self.weight.ctx._l
             return _out(self.weight.ctx, l.nrs_op_embedding(self.weight.h, _ptr(idx), idx.size, C.byref(h)), h)
@@ -444,6 +447,8 @@ class nn:
             b, s = idx.shape
             h = VP()
             l = self.weight.ctx._l
+            if self.scale is not None:
+                return _out(self.weight.ctx, l.nrs_op_embedding_scaled(self.weight.h, _ptr(idx), b, s, C.c_float(self.scale), C.byref(h)), h)
             return _out(self.weight.ctx, l.nrs_op_embedding_batch(self.weight.h, _ptr(idx), b, s, C.byref(h)), h)
 
     class PositionalEncoding:
@@ -627,8 +632,8 @@ class Trainer:
 
     `layers` uses the tuples ("conv", c_in, c_out, k, stride, pad), ("relu",), ("gelu",),
     ("maxpool", k, stride), ("flatten",), ("linear", n_in, n_out), ("batchnorm", channels),
-    ("dropout", p), ("dropout2d", p), and for token models ("embedding", vocab, d_model, max_len) as the first
-    layer, ("transformer_block", d_model, heads, d_ff, act, flags), ("layernorm", features); see
+    ("dropout", p), ("dropout2d", p), and for token models ("embedding", vocab, d_model, max_len[, 1: rows times
+    sqrt(d_model)]) as the first layer, ("transformer_block", d_model, heads, d_ff, act, flags), ("layernorm", features); see
     neuralrs_b200/workloads.py.
     """
 
