@@ -175,6 +175,20 @@ int nrs_gemm(nrs_ctx* ctx, int trans_a, int trans_b, int m, int n, int k,
 int nrs_bmm(nrs_ctx* ctx, int trans_a, int trans_b, int batch, int m, int n, int k,
             const float* a, const float* b, float* c, float beta);
 
+/* Gated feed-forward layer (no reference counterpart; the gated form of src/cuda/nn/transformer_block.rs:37):
+ *   h[m,n] = act(x[m,k] . w_gate[k,n]) * (x . w_up[k,n])
+ * both projections, the activation (any nrs_act; NONE: a product of two projections) and the product in one kernel.
+ * pre_gate, pre_up (both or neither): [m,n], the projections, which the backward pass reads.
+ * Backward: dx (+)=, and dw_gate, dw_up (+)= (both or neither); dx and the pair may be NULL.
+ * 3xTF32 mode: from 16 rows and n, k >= 32 on, f16 pairs in accumulation chains of 256 values, added up in f32: the error of
+ * an f32 product.  Fewer rows, and smaller layers: f32.  The other modes: as nrs_gemm of each product.  Like nrs_gemm, the
+ * calls use scratch of the context: graphs captured on one context are replayed one after the other. */
+int nrs_gated_linear_fwd(nrs_ctx* ctx, const float* x, const float* w_gate, const float* w_up, float* h, float* pre_gate,
+                         float* pre_up, int m, int n, int k, int act);
+int nrs_gated_linear_bwd(nrs_ctx* ctx, const float* x, const float* w_gate, const float* w_up, const float* pre_gate,
+                         const float* pre_up, const float* dh, float* dx, float* dw_gate, float* dw_up, int m, int n, int k,
+                         int act, int accumulate_x, int accumulate_w);
+
 /* y[N,Co,oh,ow] = act(conv(x[N,Ci,H,W], w[Co,Ci,kh,kw]) + b[Co]); zero padding,
  * cross-correlation, oh=(H+2p-kh)/s+1.  Replaces conv2d_im2col + matmul_nn +
  * conv2d_col2out (src/cuda/nn/conv.rs:244-279). */

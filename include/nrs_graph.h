@@ -105,6 +105,10 @@ int nrs_op_linear_act(nrs_node* x, nrs_node* w, nrs_node* b, int act, nrs_node**
 int nrs_op_conv2d_act(nrs_node* input, nrs_node* weight, nrs_node* bias, int64_t stride, int64_t pad, int act,
                       nrs_node** out);
 
+/* act(x w_gate) * (x w_up) of a gated feed-forward layer (nrs_gated_linear_fwd): x [rows, k] or [batch, seq, k], both
+ * weights [k, n], act any nrs_act.  No reference counterpart. */
+int nrs_op_gated_linear(nrs_node* x, nrs_node* w_gate, nrs_node* w_up, int act, nrs_node** out);
+
 /* Transformer pieces — src/cuda/nn/{embedding,positional,attention,multihead,
  * transformer_block}.rs.
  * Embedding::forward(indices) -> [count, dim]; the batched form -> [batch, seq, dim]

@@ -76,8 +76,16 @@ int nrs_workspace(nrs_ctx* ctx, size_t bytes, void** out) {
 
 int nrs_ws_slot(nrs_ctx* ctx, int slot, size_t bytes, void** out) {
   if (slot < 0 || slot >= NRS_WS_COUNT) return nrs_fail(ctx, NRS_ERR_ARG, "workspace: bad slot %d", slot);
+  if (bytes > ctx->ws_slot_bytes[slot] && ctx->ws_slot_captured[slot]) {
+    ctx->ws_kept.emplace_back(ctx->ws_slot[slot], ctx->ws_slot_bytes[slot]);
+    ctx->ws_slot[slot] = nullptr;
+    ctx->ws_slot_bytes[slot] = 0;
+    ctx->ws_slot_captured[slot] = false;
+  }
   const int st = grow_block(ctx, "workspace slot", bytes, &ctx->ws_slot[slot], &ctx->ws_slot_bytes[slot]);
   *out = ctx->ws_slot[slot];
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  if (st == NRS_OK && cudaStreamIsCapturing(ctx->stream, &capturing) == cudaSuccess && capturing != cudaStreamCaptureStatusNone) ctx->ws_slot_captured[slot] = true;
   return st;
 }
 
@@ -458,6 +466,7 @@ int nrs_destroy(nrs_ctx* ctx) {
   cudaStreamSynchronize(ctx->stream);
   drop_block(ctx, &ctx->workspace, &ctx->workspace_bytes);
   for (int i = 0; i < NRS_WS_COUNT; ++i) drop_block(ctx, &ctx->ws_slot[i], &ctx->ws_slot_bytes[i]);
+  for (auto& kv : ctx->ws_kept) drop_block(ctx, &kv.first, &kv.second);
   nrs_folds_free(ctx);
   nrs_weight_set_clear(ctx);
   for (auto& kv : ctx->pool.free_blocks) if (kv.first > NrsPool::kSmall) cudaFree(kv.second);

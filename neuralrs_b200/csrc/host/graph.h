@@ -223,6 +223,9 @@ NodeP causal_mask(const NodeP& scores);
 // softmax(Q K^T / sqrt(d_head)) V on [batch, seq, d_head]  (attention.rs:23-32).
 NodeP attention_batch(const NodeP& q, const NodeP& k, const NodeP& v, bool causal = false);
 
+// act(x w_gate) * (x w_up) on [rows, k] or [batch, seq, k] (nrs_gated_linear_fwd); no reference counterpart.
+NodeP gated_linear(const NodeP& x, const NodeP& w_gate, const NodeP& w_up, int act);
+
 struct Linear {                       // linear.rs:11-26
   NodeP weights, bias;
   NodeP forward(const NodeP& x) const;

@@ -373,6 +373,13 @@ int nrs_op_mha(nrs_node* x, nrs_node* w_q, nrs_node* w_k, nrs_node* w_v, nrs_nod
   });
 }
 
+int nrs_op_gated_linear(nrs_node* x, nrs_node* w_gate, nrs_node* w_up, int act, nrs_node** out) {
+  NODE_OK(x);
+  NODE_OK(w_gate);
+  NODE_OK(w_up);
+  return wrap(ctx_of(x), out, [&] { return nrs::cuda::gated_linear(x->p, w_gate->p, w_up->p, act); });
+}
+
 int nrs_rotary_new(nrs_ctx* ctx, int64_t rot_dim, int64_t max_len, float base, nrs_node** table_out) {
   NRS_REQUIRE_CTX(ctx);
   NRS_REQUIRE(ctx, rot_dim > 0 && max_len > 0, NRS_ERR_SHAPE, "nrs_rotary_new: non-positive size");

@@ -468,6 +468,65 @@ NodeP MultiHeadAttention::forward_batch(const NodeP& x) const {
   return reshape(matmul(reshape(concat, {batch * seq, d}), w_o), {batch, seq, d});
 }
 
+NodeP gated_linear(const NodeP& x, const NodeP& w_gate, const NodeP& w_up, int act) {
+  for (const NodeP& n : {x, w_gate, w_up})
+    if (!n || !n->on_gpu()) fail(NRS_ERR_ARG, "cuda gated linear: operand not on GPU");
+  if (w_gate->ctx != x->ctx || w_up->ctx != x->ctx) fail(NRS_ERR_ARG, "cuda gated linear: nodes of different contexts");
+  if ((x->shape.size() != 2 && x->shape.size() != 3) || w_gate->shape.size() != 2 || w_up->shape != w_gate->shape || w_gate->shape[0] != x->shape.back())
+    fail(NRS_ERR_SHAPE, "cuda gated linear: x must be [.., k] and both weights [k, n]");
+  const size_t k = w_gate->shape[0], n = w_gate->shape[1], m = k ? x->len() / k : 0;
+  if (k == 0 || n == 0 || m > 2147483647u || n > 2147483647u || k > 2147483647u) fail(NRS_ERR_SHAPE, "cuda gated linear: empty or too large");
+  nrs_ctx* ctx = x->ctx;
+  std::vector<size_t> shape = x->shape;
+  shape.back() = n;
+  NodeP out = make_result(ctx, shape, {x, w_gate, w_up});
+  float* pre[2];
+  for (float*& p : pre) {
+    void* q = nullptr;
+    check(ctx, nrs_alloc(ctx, std::max<size_t>(1, m * n) * sizeof(float), 0, &q));
+    out->saved.push_back(q);
+    p = (float*)q;
+  }
+  check(ctx, nrs_gated_linear_fwd(ctx, x->data, w_gate->data, w_up->data, out->data, pre[0], pre[1], (int)m, (int)n, (int)k, act));
+  Node* self = out.get();
+  float *pg = pre[0], *pu = pre[1];
+  out->backward_fn = [self, x, w_gate, w_up, pg, pu, m, n, k, act]() {
+    nrs_ctx* ctx = self->ctx;
+    const bool weights = w_gate->requires_grad || w_up->requires_grad;
+    if (!x->requires_grad && !weights) return;
+    const float* dh = grad_view(self);
+    GradSlot tx{nullptr, 0};
+    if (x->requires_grad) tx = grad_slot(x);
+    // Both weights' gradients come from one product, written or added alike.  Where only one of them is wanted, or they are
+    // at different shares (or one tensor), they go by way of scratch.
+    GradSlot t[2] = {{nullptr, 0}, {nullptr, 0}};
+    const NodeP w[2] = {w_gate, w_up};
+    for (int i = 0; i < 2; ++i)
+      if (w[i]->requires_grad) t[i] = grad_slot(w[i]);
+    const bool direct = t[0].ptr && t[1].ptr && t[0].ptr != t[1].ptr && t[0].accumulate == t[1].accumulate;
+    struct Scratch {
+      nrs_ctx* ctx;
+      float* p;
+      ~Scratch() { if (p) nrs_free(ctx, p); }
+    } scratch{ctx, nullptr};
+    const size_t len = k * n, each = (len + 63) / 64 * 64;
+    float* d[2] = {t[0].ptr, t[1].ptr};
+    if (weights && !direct) {
+      void* q = nullptr;
+      check(ctx, nrs_alloc(ctx, 2 * each * sizeof(float), 0, &q));
+      scratch.p = d[0] = (float*)q;
+      d[1] = d[0] + each;
+    }
+    check(ctx, nrs_gated_linear_bwd(ctx, x->data, w_gate->data, w_up->data, pg, pu, dh, tx.ptr, weights ? d[0] : nullptr, weights ? d[1] : nullptr, (int)m,
+                                    (int)n, (int)k, act, tx.accumulate, direct ? t[0].accumulate : 0));
+    if (!scratch.p) return;
+    check(ctx, nrs_folds_flush(ctx));
+    for (int i = 0; i < 2; ++i)
+      if (t[i].ptr) check(ctx, t[i].accumulate ? nrs_accumulate(ctx, t[i].ptr, d[i], len) : nrs_d2d(ctx, t[i].ptr, d[i], len * sizeof(float)));
+  };
+  return out;
+}
+
 static NodeP block_body(const TransformerBlock& b, const NodeP& x, bool final_norm) {
   if (!x || x->shape.size() != 3) fail(NRS_ERR_SHAPE, "cuda transformer block: input must be [batch, seq, d_model]");
   const size_t batch = x->shape[0], seq = x->shape[1], d = x->shape[2];

@@ -231,8 +231,10 @@ struct nrs_ctx {
   void* workspace = nullptr;
   size_t workspace_bytes = 0;
   // Named grow-only scratch blocks (operand staging for the tensor-core kernels).
-  void* ws_slot[5] = {nullptr, nullptr, nullptr, nullptr, nullptr};
-  size_t ws_slot_bytes[5] = {0, 0, 0, 0, 0};
+  void* ws_slot[6] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+  size_t ws_slot_bytes[6] = {0, 0, 0, 0, 0, 0};
+  bool ws_slot_captured[6] = {};     // a captured graph may use the block: it is kept when the slot grows
+  std::vector<std::pair<void*, size_t>> ws_kept;
   // Device word the tensor-core kernels set when a bounded wait runs out; read at sync points.
   int* err_flag = nullptr;
   volatile int* err_host = nullptr;  // the same word as the host sees it (mapped memory)
@@ -304,7 +306,7 @@ int nrs_device_alloc(nrs_ctx* ctx, const char* what, size_t bytes, void** out);
 int nrs_workspace(nrs_ctx* ctx, size_t bytes, void** out);
 // (the weight-gradient kernels keep their split partials in a slot of their own: they may run while the
 // data gradient's K-split is still being folded out of NRS_WS_PARTIAL)
-enum { NRS_WS_A = 0, NRS_WS_B = 1, NRS_WS_PARTIAL = 2, NRS_WS_WGRAD_PARTIAL = 3, NRS_WS_FOLD = 4, NRS_WS_COUNT = 5 };
+enum { NRS_WS_A = 0, NRS_WS_B = 1, NRS_WS_PARTIAL = 2, NRS_WS_WGRAD_PARTIAL = 3, NRS_WS_FOLD = 4, NRS_WS_GATED = 5, NRS_WS_COUNT = 6 };
 int nrs_ws_slot(nrs_ctx* ctx, int slot, size_t bytes, void** out);
 // Room for operand planes of `values` values in one slot (with `split` both of a pair in one block); *lo is null without.
 int nrs_ws_planes(nrs_ctx* ctx, int slot, size_t values, bool split, void** hi, void** lo);

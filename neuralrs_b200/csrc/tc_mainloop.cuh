@@ -56,6 +56,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "igemm_problems.cuh"
 #include "nrs_internal.h"
@@ -109,11 +110,20 @@ struct Ranges {
   NrsRange* out;
 };
 
+// Policies with a kChainK (gated layers) accumulate no more than that many values of K in the tensor core: the epilogue warps
+// keep a tile's sums in registers (a warp's share of 128 x 128 is 32 values a lane) and add each chain to them in f32, under
+// the next chain's products.  At 256 the error is that of an f32 product (3.5e-7 against 64 bits; 4.9e-6 in a chain of 4096).
+template <class Policy, class = void>
+struct ShortChains : std::false_type {};
+template <class Policy>
+struct ShortChains<Policy, std::void_t<decltype(Policy::kChainK)>> : std::true_type {};
+
 struct SplitInfo {
   int splits;          // K-splits per (tile, batch)
   int kb_per_split;    // K-slices per split, or per chunk
   int chunks;          // > 1 (splits == 1 then): K-chunks that a CTA takes one after the other
   int kb_total;        // K-slices in all
+  int kb_chain;        // ShortChains: K-slices of one chain
   int batches;
   NrsFastDiv div_splits;
   float* partial;      // [split][batch][tiles_m*128][n_total] when splits > 1; [CTA][128][BN] when chunks > 1
@@ -453,8 +463,9 @@ tc_kernel(const __grid_constant__ CUtensorMap tm_a_hi, const __grid_constant__ C
         const int split = z - (int)sp.div_splits.div((uint32_t)z) * sp.splits;
         int kb_begin = split * sp.kb_per_split, kb_end = sp.chunks > 1 ? sp.kb_total : min(sp.kb_total, kb_begin + sp.kb_per_split);
         if (!pol.clip(tile_m, tile_n, BN, &kb_begin, &kb_end)) continue;
-        for (int k0 = kb_begin; k0 < kb_end && ok; k0 += sp.kb_per_split) {
-          const int nkb = min(sp.kb_per_split, kb_end - k0);   // >= 1 by construction
+        const int chain = ShortChains<Policy>::value ? sp.kb_chain : sp.kb_per_split;
+        for (int k0 = kb_begin; k0 < kb_end && ok; k0 += chain) {
+          const int nkb = min(chain, kb_end - k0);   // >= 1 by construction
           const uint32_t buf = local & 1u, use = local >> 1;
           ++local;
           if (!(PAIR ? mbar_wait_warp_cluster(&acc_empty[buf], (use & 1u) ^ 1u) : mbar_wait_warp(&acc_empty[buf], (use & 1u) ^ 1u))) { ok = false; break; }
@@ -543,6 +554,69 @@ tc_kernel(const __grid_constant__ CUtensorMap tm_a_hi, const __grid_constant__ C
       const int c_first = E::first(warp - 2);
       // What the first block reads besides the accumulator is under way before that is full.
       [[maybe_unused]] auto extra = pol.template fetch<kW>(rw, n0 + c_first * kW, E::reads_first(c_first, n0, sp.n_total, sp.splits));
+      if constexpr (ShortChains<Policy>::value) {
+        constexpr int kMine = kBlocks / kStep > 0 ? kBlocks / kStep : 1;   // column blocks of a warp
+        float sums[kMine][kW];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+#pragma unroll
+          for (int j = 0; j < kW; ++j) sums[i][j] = 0.0f;
+        const bool takes_part = c_first < kBlocks && !(PAIR && tile_m * BM >= sp.rows_total);
+        for (int k0 = kb_begin; k0 < kb_end && ok; k0 += sp.kb_chain) {
+          const uint32_t buf = local & 1u, use = local >> 1;
+          ++local;
+          if (!mbar_wait_warp(&acc_full[buf], use & 1u)) {
+            if (lane == 0) atomicExch(err_flag, kErrEpilogueWait);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t acc = tmem_base + buf * (uint32_t)L::kAccCols + ((uint32_t)(q * 32) << 16);
+          if (takes_part) {
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+              uint32_t r[kW], r2[kW];
+              const int c = c_first + i * kStep;
+              tmem_ld_32(acc + (uint32_t)(c * kW), r);
+              tmem_ld_32(acc + (uint32_t)(BN + c * kW), r2);
+              tmem_ld_wait();
+              unscale.apply(r, r2);
+#pragma unroll
+              for (int j = 0; j < kW; ++j) sums[i][j] += __uint_as_float(r[j]);
+            }
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {   // to the issuing thread, which a pair has in rank 0
+            if constexpr (PAIR) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0)); else mbar_arrive(&acc_empty[buf]);
+          }
+        }
+        if (!ok) break;
+        if (!takes_part) continue;
+        float* scratch = reinterpret_cast<float*>(emit_tile) + (warp - 2) * 512;
+        const int r0 = q * 32 + (lane >> 2);
+        if constexpr (Policy::kGated) {
+          pol.template finish<kMine>(tile_m, tile_n, c_first, r0, lane, scratch, sums, top);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            const int c = c_first + i * kStep, n = n0 + c * kW + (lane & 3) * 4;
+            if (n0 + c * kW >= sp.n_total) continue;
+            uint32_t r[kW];
+#pragma unroll
+            for (int j = 0; j < kW; ++j) r[j] = __float_as_uint(sums[i][j]);
+            float4 v[4];
+            rows_to_lines(scratch, lane, r, v);
+            if (sp.splits > 1) {
+              float* dst = sp.partial + (((size_t)split * sp.batches + batch) * sp.rows_total + (size_t)tile_m * BM + r0) * sp.n_total + n;
+#pragma unroll
+              for (int j = 0; j < 4; ++j, dst += (size_t)8 * sp.n_total) store_guarded(dst, v[j], sp.n_total - n, sp.n_total % 4 == 0);
+            } else {
+              pol.epilogue(tile_m, r0, n, v);
+            }
+          }
+        }
+      } else
       for (int k0 = kb_begin; k0 < kb_end && ok; k0 += sp.kb_per_split) {
         const uint32_t buf = local & 1u, use = local >> 1;
         ++local;
@@ -824,12 +898,17 @@ int launch(nrs_ctx* ctx, const CUtensorMap& ta_hi, const CUtensorMap& ta_lo, con
   const int tiles_n = (n_total + BN - 1) / BN;
   SplitInfo sp{};
   if (Policy::kMaySplit) {
-    plan_split(ctx, (long)tiles_m * tiles_n * batches, (long)tiles_m * BM * n_total * batches, kb_total, k_per_block, NPLANES == 2, Policy::kConv, &sp);
+    plan_split(ctx, (long)tiles_m * tiles_n * batches, (long)tiles_m * BM * n_total * batches, kb_total, k_per_block,
+               NPLANES == 2 && !ShortChains<Policy>::value, Policy::kConv, &sp);
   } else {   // tiles whose K ranges differ
     sp.splits = sp.chunks = 1;
     sp.kb_per_split = kb_total;
   }
   sp.kb_total = kb_total;
+  if constexpr (ShortChains<Policy>::value) {
+    static_assert(NPLANES == 2 && KW == 64 && BN >= 64 && !Policy::kSlab && !Policy::kCanEmit, "f16 pairs, slices of 64");
+    sp.kb_chain = Policy::kChainK / KW;
+  }
   sp.div_splits = NrsFastDiv(sp.splits);
   sp.batches = batches;
   sp.n_total = n_total;

@@ -413,6 +413,13 @@ class nn:
         return _out(x.ctx, x.ctx._l.nrs_op_linear_act(x.h, w.h, b.h, int(act), C.byref(h)), h)
 
     @staticmethod
+    def gated_linear(x: Node, w_gate: Node, w_up: Node, act: int) -> Node:
+        """act(x w_gate) * (x w_up), the inner part of a gated feed-forward layer (act: _lib.ACT_*; no reference
+        counterpart)."""
+        h = VP()
+        return _out(x.ctx, x.ctx._l.nrs_op_gated_linear(x.h, w_gate.h, w_up.h, int(act), C.byref(h)), h)
+
+    @staticmethod
     def attention_batch(q: Node, k: Node, v: Node, causal: bool = False) -> Node:
         """src/cuda/nn/attention.rs:23-32 (causal is an extension)."""
         h = VP()
