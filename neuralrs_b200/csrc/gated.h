@@ -5,23 +5,27 @@
 
 namespace gated {
 
-// exp(-a), kept finite
-__device__ __forceinline__ float exp_minus(float a) { return expf(fminf(-a, 80.0f)); }
-
-__device__ __forceinline__ float act(float a, int kind) {
-  if (kind == NRS_ACT_SILU) return a / (1.0f + exp_minus(a));
-  return nrs_apply_act(a, kind);
+// 1 / (1 + exp(-v)), and exp(-v) itself, kept finite.  The exponential as a power of two, 2 ulp, of -v log2(e) taken in two
+// parts (its rounding error is put back to first order), and the quotient within 2 ulp: a third of the instructions that
+// expf and a correctly rounded division take, which is what these element-wise passes were bound by.
+__device__ __forceinline__ float sigmoid(float v, float& e) {
+  constexpr float kLog2e = 1.4426950408889634f, kRest = (float)(1.4426950408889634 - (double)kLog2e), kLn2 = 0.6931471805599453f;
+  const float x = fmaxf(fminf(-v, 80.0f), -120.0f), t = x * kLog2e, rest = fmaf(x, kRest, fmaf(x, kLog2e, -t));
+  const float p = exp2f(t);
+  e = fmaf(p, rest * kLn2, p);
+  return __fdividef(1.0f, 1.0f + e);
 }
-// act(a) and its derivative.  SiLU: s (1 + a (1 - s)) with s = 1 / (1 + e), e = exp(-a), and 1 - s = e s, which cancels
-// nowhere.
+// act(a) and its derivative.  SiLU is a s with s = sigmoid(a), GELU (the tanh form) with s = sigmoid(2 u), u = sqrt(2/pi) (a +
+// 0.044715 a^3); with w the sigmoid's argument the derivative is s + a s (1 - s) dw/da, and 1 - s = e s cancels nowhere.
 __device__ __forceinline__ void act_both(float a, int kind, float& f, float& d) {
-  if (kind == NRS_ACT_SILU) {
-    const float e = exp_minus(a), s = 1.0f / (1.0f + e);
+  if (kind == NRS_ACT_SILU || kind == NRS_ACT_GELU) {
+    const float a2 = a * a;
+    const float w = kind == NRS_ACT_SILU ? a : 1.5957691216f * a * fmaf(0.044715f, a2, 1.0f);
+    const float dw = kind == NRS_ACT_SILU ? 1.0f : 1.5957691216f * fmaf(3.0f * 0.044715f, a2, 1.0f);
+    float e;
+    const float s = sigmoid(w, e);
     f = a * s;
-    d = s * fmaf(a, e * s, 1.0f);
-  } else if (kind == NRS_ACT_GELU) {
-    f = nrs_gelu_f(a);
-    d = nrs_gelu_d(a);
+    d = e > 0.0f ? fmaf(f * (e * s), dw, s) : 1.0f;   // (e == 0: a far to the right, where a dw may leave f32's range)
   } else if (kind == NRS_ACT_RELU) {
     f = a > 0.0f ? a : 0.0f;
     d = a > 0.0f ? 1.0f : 0.0f;
@@ -29,6 +33,11 @@ __device__ __forceinline__ void act_both(float a, int kind, float& f, float& d) 
     f = a;
     d = 1.0f;
   }
+}
+__device__ __forceinline__ float act(float a, int kind) {
+  float f, d;
+  act_both(a, kind, f, d);
+  return f;
 }
 
 struct Shape { int m, n, k, act; };

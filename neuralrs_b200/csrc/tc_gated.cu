@@ -6,8 +6,12 @@
 //
 // Main loop: tc_mainloop.cuh, f16 pairs (3xTF32), chains of 256 values of K summed in registers.  Forward, a tile's 128
 // columns are 64 of a and the same 64 of u, so a warp that has both in its registers multiplies them where they are: neither
-// leaves the SM unless the backward pass needs it.  (A pair of CTAs brings the 64 rows of Wg^T in one and of Wu^T in the
-// other.)
+// leaves the SM unless the backward pass needs it.  (Of a pair of CTAs, one brings the columns of Wg and one those of Wu.)
+//
+// Operand planes: every tensor as it is stored, rows padded with zeros to a multiple of 64 values, Wg and Wu (da and du) side
+// by side in one row.  The forward product reads the weights' planes with k across the rows, dx along them, the weight
+// gradients x and da|du across: nothing is transposed (staging 2048 x 5504 weights transposed took 112 us, as they are 36).
+// All of a pass's operands are measured by one launch and written by another.
 #include "gated.h"
 #include "tc_mainloop.cuh"
 
@@ -20,7 +24,7 @@ enum Product { kForward, kInput, kWeights };
 template <Product P>
 struct GatedPolicy {
   static constexpr bool kCanEmit = false, kConv = false, kSlab = false;
-  static constexpr bool kGated = P == kForward, kAMnMajor = P == kWeights, kBMnMajor = P == kWeights;
+  static constexpr bool kGated = P == kForward, kAMnMajor = P == kWeights, kBMnMajor = P != kInput;
   static constexpr bool kMaySplit = P != kForward;
   static constexpr int kEpiWarps = 16, kTeamWarps = 4;
   static constexpr int kChainK = 256;
@@ -29,7 +33,7 @@ struct GatedPolicy {
   float* out[2];         // forward: h; input: dx; weights: dWg, dWu
   float* pre[2];         // forward: a, u, or null
   int M, N;              // of the output as it is stored (weights: of one matrix)
-  int ld;                // weights: columns of one matrix in the product, padding included; input: columns of da, likewise
+  int ld;                // n, padded: columns of one of the two matrices side by side
   int act, accumulate;
   bool vec;              // rows of the outputs start on 16 bytes
 
@@ -59,10 +63,10 @@ struct GatedPolicy {
     } else if (P == kInput) {
       tc::tma_load_3d_to<PAIR>(dst, tm, bar, c.col, n0, c.mat);
     } else if (PAIR) {           // half of the tile's columns: this CTA's matrix
-      tc::tma_load_3d_to<PAIR>(dst, tm, bar, c.col, n0 / BN * (BN / 2), n0 % BN != 0);
+      tc::tma_load_3d_to<PAIR>(dst, tm, bar, 0, c.col, n0 / BN + (n0 % BN != 0 ? ld / 64 : 0));
     } else {
-      tc::tma_load_3d_to<PAIR>(dst, tm, bar, c.col, n0 / 2, 0);
-      tc::tma_load_3d_to<PAIR>(reinterpret_cast<uint8_t*>(dst) + BN / 2 * ROW_BYTES, tm, bar, c.col, n0 / 2, 1);
+      tc::tma_load_3d_to<PAIR>(dst, tm, bar, 0, c.col, n0 / BN);
+      tc::tma_load_3d_to<PAIR>(reinterpret_cast<uint8_t*>(dst) + BN / 2 * ROW_BYTES, tm, bar, 0, c.col, n0 / BN + ld / 64);
     }
   }
   __device__ __forceinline__ float out_bound(float, float, int) const { return 0.0f; }
@@ -72,46 +76,28 @@ struct GatedPolicy {
 
   // Forward: a warp's 32 rows of 16 columns of a (sums[0]) and of u (sums[1]).
   template <int MINE>
-  __device__ __forceinline__ void finish(int tile_m, int tile_n, int c, int r0, int lane, float* scratch, float (&sums)[MINE][16], uint32_t&) const {
+  __device__ __forceinline__ void finish(int m0, int tile_n, int c, int lane, float* scratch, float (&sums)[MINE][16]) const {
     static_assert(MINE == 2, "the columns of both matrices");
-    const int n = tile_n * 64 + c * 16 + (lane & 3) * 4, m0 = tile_m * tc::BM + r0, left = N - n;
-    if (tile_n * 64 + c * 16 >= N) return;
-    uint32_t r[16];
-    float4 v[4];
-    auto send = [&](float* dst) {
-      tc::rows_to_lines(scratch, lane, r, v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (m0 + 8 * i < M) tc::store_guarded(dst + (size_t)(m0 + 8 * i) * N + n, v[i], left, vec);
-    };
+    const int n = tile_n * 64 + c * 16;
+    if (n >= N) return;
+    const size_t at = (size_t)m0 * N + n;
     if (pre[0]) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(sums[s][j]);
-        send(pre[s]);
-      }
+      send(pre[0] + at, m0, n, lane, scratch, sums[0]);
+      send(pre[1] + at, m0, n, lane, scratch, sums[1]);
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(gated::act(sums[0][j], act) * sums[1][j]);
-    send(out[0]);
+    for (int j = 0; j < 16; ++j) sums[0][j] = gated::act(sums[0][j], act) * sums[1][j];
+    send(out[0] + at, m0, n, lane, scratch, sums[0]);
   }
-
-  // Four row segments of the output, rows r0 + 8 i of the tile, columns n..n+3.
-  __device__ __forceinline__ void epilogue(int tile_m, int r0, int n, const float4 (&v)[4]) const {
-    const int mat = P == kWeights && n >= ld ? 1 : 0, c = n - mat * ld, left = N - c, m0 = tile_m * tc::BM + r0;
-    if (left <= 0) return;
-    float* dst = out[mat] + (size_t)m0 * N + c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i, dst += (size_t)8 * N) {
-      if (m0 + 8 * i >= M) return;
-      float4 q = v[i];
-      if (accumulate) {
-        const float4 o = tc::load_guarded(dst, left, vec);
-        q = make_float4(o.x + q.x, o.y + q.y, o.z + q.z, o.w + q.w);
-      }
-      tc::store_guarded(dst, q, left, vec);
-    }
+  __device__ __forceinline__ void send(float* dst, int m0, int n, int lane, float* scratch, const float (&v)[16]) const {
+    if (vec) tc::block_to_rows<true>(scratch, lane, v, dst, N, M - m0, N - n, accumulate != 0);
+    else tc::block_to_rows<false>(scratch, lane, v, dst, N, M - m0, N - n, accumulate != 0);
+  }
+  // 32 rows from m0 on and 16 columns from n on of the product.
+  __device__ __forceinline__ void block(int m0, int n, int lane, float* scratch, const float (&v)[16]) const {
+    const int mat = P == kWeights && n >= ld ? 1 : 0, c = n - mat * ld;
+    if (c >= N) return;
+    send(out[mat] + (size_t)m0 * N + c, m0, c, lane, scratch, v);
   }
   // One element, from the pass that sums a K-split.
   template <bool SPLIT>
@@ -123,212 +109,259 @@ struct GatedPolicy {
   }
 };
 
-// ------------------------------------------------------------------------------------------------ da and du
+// ------------------------------------------------------------------------------------------------ operand planes
 
-// Four values of da and du.
-__device__ __forceinline__ void gradients(float4 g, float4 a, float4 u, int kind, float4& da, float4& du) {
-  const float gg[4] = {g.x, g.y, g.z, g.w}, aa[4] = {a.x, a.y, a.z, a.w}, uu[4] = {u.x, u.y, u.z, u.w};
-  float p[4], q[4];
+// A tensor [rows][cols] on its way to planes, or (a, u given) the two that dh, a and u make, da and du.
+struct Job {
+  const float* src;
+  const float *a, *u;
+  __half *hi, *lo;
+  NrsRange* range;
+  int rows, cols, pad;      // pad: a row's values in the planes, cols rounded up to 64
+  long ld;                  // values between rows of the planes
+  unsigned first, blocks;   // of the launch
+  NrsFastDiv div;           // of pad / 8
+  bool vec;
+};
+struct Jobs {
+  Job j[4];
+  int count, act;
+};
+
+__device__ __forceinline__ void eight(float (&v)[8], const float* p, int left, bool vec) {
+  if (vec && left >= 8) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float f, d;
-    gated::act_both(aa[j], kind, f, d);
-    p[j] = gg[j] * uu[j] * d;
-    q[j] = gg[j] * f;
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.0f;
   }
-  da = make_float4(p[0], p[1], p[2], p[3]);
-  du = make_float4(q[0], q[1], q[2], q[3]);
+}
+__device__ __forceinline__ void put8(__half* hi, __half* lo, size_t at, const float (&v)[8], float scale) {
+  uint2 h0, l0, h1, l1;
+  pr::split4(make_float4(v[0], v[1], v[2], v[3]), scale, &h0, &l0);
+  pr::split4(make_float4(v[4], v[5], v[6], v[7]), scale, &h1, &l1);
+  *reinterpret_cast<uint4*>(hi + at) = make_uint4(h0.x, h0.y, h1.x, h1.y);
+  *reinterpret_cast<uint4*>(lo + at) = make_uint4(l0.x, l0.y, l1.x, l1.y);
 }
 
-// Two passes over dh, a and u: the largest magnitude of what they give (WRITE == false), then the pairs
-// [m][da: ld | du: ld], zeros from n to ld.
-template <bool WRITE>
-__global__ void __launch_bounds__(256)
-gated_planes_kernel(const float* __restrict__ g, const float* __restrict__ a, const float* __restrict__ u, float* hi, float* lo, NrsRange* range, int m, int n,
-                    int ld, NrsFastDiv div /*of ld / 4*/, int kind, bool vec) {
+// MEASURE: the largest magnitude of each tensor into its range.  Of da and du: of dh u, times 1.13, which no activation's
+// slope exceeds, and of dh a, which no activation exceeds; without their exponentials this is a pass at memory speed.
+// Otherwise the pairs, zeros from cols to pad.
+template <bool MEASURE>
+__global__ void __launch_bounds__(256) gated_stage_kernel(const Jobs jobs) {
   NRS_PDL_PROLOGUE();
-  const uint32_t quads = (uint32_t)m * (uint32_t)(ld / 4), stride = gridDim.x * blockDim.x;   // (the launcher checks the range)
-  float scale = 1.0f;
-  if (WRITE) {
-    const float bound = range->top;
-    scale = pr::scale_of(bound);
-    if (blockIdx.x == 0 && threadIdx.x == 0) range->bound = bound;
-  }
+  int which = 0;
+  while (which + 1 < jobs.count && blockIdx.x >= jobs.j[which + 1].first) ++which;
+  const Job& q = jobs.j[which];
+  const uint32_t units = (uint32_t)q.rows * (uint32_t)(q.pad / 8), step = q.blocks * 256;   // (the launcher checks the range)
+  const bool grads = q.a != nullptr;
+  const float bound = MEASURE ? 0.0f : q.range->top, scale = MEASURE ? 1.0f : pr::scale_of(bound);
+  if (!MEASURE && blockIdx.x == q.first && threadIdx.x == 0) q.range->bound = bound;
   uint32_t top = 0;
   constexpr int kDeep = 2;
-  for (uint32_t i0 = blockIdx.x * blockDim.x + threadIdx.x; i0 < quads; i0 += kDeep * stride) {
-    float4 vg[kDeep], va[kDeep], vu[kDeep];
-    uint32_t row[kDeep], q[kDeep];
+  for (uint32_t i0 = (blockIdx.x - q.first) * 256 + threadIdx.x; i0 < units; i0 += kDeep * step) {
+    float g[kDeep][8], a[kDeep][8], u[kDeep][8];
+    uint32_t row[kDeep], col[kDeep];
 #pragma unroll
     for (int k = 0; k < kDeep; ++k) {
-      const uint32_t i = i0 + k * stride;
-      vg[k] = va[k] = vu[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (i >= quads) continue;
-      div.divmod(i, row[k], q[k]);
-      const int left = n - (int)(4 * q[k]);
-      if (left <= 0) continue;
-      const size_t at = (size_t)row[k] * n + 4 * q[k];
-      vg[k] = tc::load_guarded(g + at, left, vec);
-      va[k] = tc::load_guarded(a + at, left, vec);
-      vu[k] = tc::load_guarded(u + at, left, vec);
+      const uint32_t i = min(i0 + k * step, units - 1);   // (past the end: the last one again)
+      q.div.divmod(i, row[k], col[k]);
+      col[k] *= 8;
+      const int left = q.cols - (int)col[k];
+      const size_t at = (size_t)row[k] * q.cols + col[k];
+      eight(g[k], q.src + at, left, q.vec);
+      if (grads) {
+        eight(a[k], q.a + at, left, q.vec);
+        eight(u[k], q.u + at, left, q.vec);
+      }
     }
 #pragma unroll
     for (int k = 0; k < kDeep; ++k) {
-      if (i0 + k * stride >= quads) continue;
-      float4 da, du;
-      gradients(vg[k], va[k], vu[k], kind, da, du);
-      if (WRITE) {
-        const size_t at = (size_t)row[k] * (2 * ld) + 4 * q[k];
-        pr::put4(hi, lo, at, da, scale);
-        pr::put4(hi, lo, at + ld, du, scale);
+      if (k > 0 && i0 + k * step >= units) break;
+      const size_t at = (size_t)row[k] * q.ld + col[k];
+      if (MEASURE) {
+        if (grads) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            u[k][i] *= 1.13f * g[k][i];
+            a[k][i] *= g[k][i];
+          }
+          top = pr::seen_all(top, u[k]);
+          top = pr::seen_all(top, a[k]);
+        } else {
+          top = pr::seen_all(top, g[k]);
+        }
+      } else if (grads) {
+        float da[8], du[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float f, d;
+          gated::act_both(a[k][i], jobs.act, f, d);
+          da[i] = g[k][i] * u[k][i] * d;
+          du[i] = g[k][i] * f;
+        }
+        put8(q.hi, q.lo, at, da, scale);
+        put8(q.hi, q.lo, at + q.pad, du, scale);
       } else {
-        top = pr::seen4(top, da);
-        top = pr::seen4(top, du);
+        put8(q.hi, q.lo, at, g[k], scale);
       }
     }
   }
-  if (!WRITE) {
+  if (MEASURE) {
     __syncwarp();
-    pr::report(range, top);
+    pr::report(q.range, top);
   }
 }
-
-struct Planes {
-  void *hi, *lo;
-  const NrsRange* range;
-};
 
 int round64(int v) { return (v + 63) / 64 * 64; }
 
-// [batch][rows][cols] planes with rows ld values apart, cols values of K a row.
-bool map_k(CUtensorMap* t, const void* base, int cols, int rows, int batch, size_t ld, size_t bstride, int box_rows) {
-  const uint64_t dim[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)batch}, str[2] = {ld, bstride};
-  const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
-  return tc::encode_tmap(t, base, true, 3, dim, str, box);
+struct Planes {
+  void *hi, *lo;
+  NrsRange* range;
+  int pad, ld;              // values of one matrix in a row, and of a row
+};
+int open_planes(nrs_ctx* ctx, int slot, int rows, int cols, int side_by_side, Planes* out) {
+  out->pad = round64(cols);
+  out->ld = side_by_side * out->pad;
+  const int st = nrs_ws_planes(ctx, slot, (size_t)rows * out->ld, true, &out->hi, &out->lo);
+  return st == NRS_OK ? nrs_range_renew(ctx, out->hi, &out->range) : st;
 }
-// Rows of K: [row block of 64 columns][k][64].
-bool map_mn(CUtensorMap* t, const void* base, int cols /*a multiple of 64*/, int k, int box_cols) {
-  const uint64_t dim[3] = {64, (uint64_t)k, (uint64_t)(cols / 64)}, str[2] = {(uint64_t)cols, 64};
-  const uint32_t box[3] = {64, 64, (uint32_t)(box_cols / 64)};
-  return tc::encode_tmap(t, base, true, 3, dim, str, box, true);
-}
-
-template <int BN, bool PAIR, Product P>
-int run(nrs_ctx* ctx, const Planes& A, const Planes& B, const GatedPolicy<P>& pol, int rows, int cols, int kdim, int a_batch, size_t a_ld, size_t a_stride,
-        int b_rows, size_t b_ld, size_t b_stride, int kblocks) {
-  constexpr int kBRows = PAIR || P == kForward ? BN / 2 : BN;   // rows of B in one load
-  CUtensorMap a[2], b[2];
-  bool ok = true;
-  for (int i = 0; i < 2; ++i) {
-    const void *pa = i ? A.lo : A.hi, *pb = i ? B.lo : B.hi;
-    if (P == kWeights) ok = ok && map_mn(&a[i], pa, (int)a_ld, kdim, tc::BM) && map_mn(&b[i], pb, (int)b_ld, kdim, kBRows);
-    else ok = ok && map_k(&a[i], pa, kdim, rows, a_batch, a_ld, a_stride, tc::BM) && map_k(&b[i], pb, kdim, b_rows, 2, b_ld, b_stride, kBRows);
-  }
-  NRS_REQUIRE(ctx, ok, NRS_ERR_CUDA, "gated layer: cuTensorMapEncodeTiled failed (%d x %d x %d)", rows, cols, kdim);
-  return tc::launch<BN, 2, PAIR, 64, GatedPolicy<P>>(ctx, a[0], a[1], b[0], b[1], pol, (rows + tc::BM - 1) / tc::BM, cols, 1, kblocks,
-                                                     tc::Ranges{A.range, B.range, nullptr});
-}
-
 bool aligned(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (reinterpret_cast<uintptr_t>(p) & 15) return false;
   return true;
 }
-
-// Planes of x [m][k] with rows round64(k) values apart.
-int stage_x(nrs_ctx* ctx, const Shape& s, const float* x, Planes* out) {
-  const int ld = round64(s.k);
-  int st = nrs_ws_planes(ctx, NRS_WS_A, (size_t)s.m * ld, true, &out->hi, &out->lo);
-  if (st == NRS_OK) st = nrs_tc_stage(ctx, x, (float*)out->hi, (float*)out->lo, s.m, s.k, ld, 1, 0, 0, false);
-  out->range = nrs_range_of(ctx, out->hi);
-  return st;
+void add_job(Jobs* jobs, const float* src, const float* a, const float* u, int rows, int cols, const Planes& to, int mat) {
+  Job& q = jobs->j[jobs->count++];
+  q.src = src; q.a = a; q.u = u;
+  q.hi = (__half*)to.hi + (size_t)mat * to.pad; q.lo = (__half*)to.lo + (size_t)mat * to.pad;
+  q.range = to.range;
+  q.rows = rows; q.cols = cols; q.pad = to.pad; q.ld = to.ld;
+  q.div = NrsFastDiv(to.pad / 8);
+  q.vec = cols % 4 == 0 && aligned({src, a, u});
 }
-// Planes of both weights, one behind the other, with one range: transposed ([n][k]), or as stored ([k][n]).
-int stage_weights(nrs_ctx* ctx, const Shape& s, const float* wg, const float* wu, bool transposed, Planes* out) {
-  const float* w[2] = {wg, wu};
-  const int rows = transposed ? s.n : s.k, cols = transposed ? s.k : s.n, ld = round64(cols);
-  int st = nrs_ws_planes(ctx, NRS_WS_B, 2 * (size_t)rows * ld, true, &out->hi, &out->lo);
-  if (st == NRS_OK) st = nrs_tc_stage_each(ctx, w, 2, (float*)out->hi, (float*)out->lo, rows, cols, ld, (size_t)rows * ld, transposed);
-  out->range = nrs_range_of(ctx, out->hi);
-  return st;
+// Blocks by the jobs' bytes, up to eight an SM in all (a job's own units permitting).
+template <bool MEASURE>
+int run_jobs(nrs_ctx* ctx, Jobs& jobs) {
+  double work[4], all = 0.0;
+  for (int i = 0; i < jobs.count; ++i) all += work[i] = (double)jobs.j[i].rows * jobs.j[i].pad * (jobs.j[i].a ? (MEASURE ? 3.0 : 5.0) : (MEASURE ? 1.0 : 2.0));
+  unsigned at = 0;
+  for (int i = 0; i < jobs.count; ++i) {
+    Job& q = jobs.j[i];
+    const unsigned most = (unsigned)(((size_t)q.rows * (q.pad / 8) + 255) / 256), share = (unsigned)(work[i] / all * 8 * ctx->sm_count) + 1;
+    q.first = at;
+    q.blocks = std::min(most, share);
+    at += q.blocks;
+  }
+  NRS_PDL_LAUNCH(gated_stage_kernel<MEASURE>, at, 256, 0, ctx->stream, jobs);
+  NRS_LAUNCHED(ctx);
+  return NRS_OK;
+}
+
+// Planes with K along the rows: [mat][row][cols].
+bool map_k(CUtensorMap* t, const void* base, const Planes& p, int cols, int rows, int mats, int box_rows) {
+  const uint64_t dim[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)mats}, str[2] = {(uint64_t)p.ld, (uint64_t)p.pad};
+  const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
+  return tc::encode_tmap(t, base, true, 3, dim, str, box);
+}
+// Planes with K across the rows: [block of 64 columns][k][64].
+bool map_mn(CUtensorMap* t, const void* base, const Planes& p, int k, int box_cols) {
+  const uint64_t dim[3] = {64, (uint64_t)k, (uint64_t)(p.ld / 64)}, str[2] = {(uint64_t)p.ld, 64};
+  const uint32_t box[3] = {64, 64, (uint32_t)(box_cols / 64)};
+  return tc::encode_tmap(t, base, true, 3, dim, str, box, true);
+}
+
+// The product of A [rows] and B [cols, padding included]; k: its length (input: of one matrix).
+template <int BN, bool PAIR, Product P>
+int run(nrs_ctx* ctx, const Planes& A, const Planes& B, const GatedPolicy<P>& pol, int rows, int cols, int k) {
+  constexpr int kBCols = PAIR || P == kForward ? BN / 2 : BN;   // of B in one load
+  CUtensorMap a[2], b[2];
+  bool ok = true;
+  for (int i = 0; i < 2; ++i) {
+    const void *pa = i ? A.lo : A.hi, *pb = i ? B.lo : B.hi;
+    ok = ok && (P == kWeights ? map_mn(&a[i], pa, A, k, tc::BM) : map_k(&a[i], pa, A, k, rows, P == kInput ? 2 : 1, tc::BM));
+    ok = ok && (P == kInput ? map_k(&b[i], pb, B, k, cols, 2, kBCols) : map_mn(&b[i], pb, B, k, kBCols));
+  }
+  NRS_REQUIRE(ctx, ok, NRS_ERR_CUDA, "gated layer: cuTensorMapEncodeTiled failed (%d x %d x %d)", rows, cols, k);
+  const int kb = P == kInput ? 2 * (A.pad / 64) : (k + 63) / 64;
+  return tc::launch<BN, 2, PAIR, 64, GatedPolicy<P>>(ctx, a[0], a[1], b[0], b[1], pol, (rows + tc::BM - 1) / tc::BM, cols, 1, kb,
+                                                     tc::Ranges{A.range, B.range, nullptr});
 }
 
 bool applies(const nrs_ctx* ctx, const Shape& s) {
-  // (from 16 rows on, as the ungated products; the elementwise passes count quads in 32 bits)
-  return ctx->math_mode == NRS_MATH_3XTF32 && tc::tensor_map_encoder() && s.m >= 16 && s.n >= 32 && s.k >= 32 &&
-         (uint64_t)s.m * (uint64_t)(round64(s.n) / 4) < 0x40000000ull && s.n <= (1 << 24) && s.k <= (1 << 24);
+  // (from 16 rows on, as the ungated products; the staging passes count eights in 32 bits)
+  const uint64_t m = s.m, n = round64(s.n), k = round64(s.k), most = 1ull << 33;
+  return ctx->math_mode == NRS_MATH_3XTF32 && tc::tensor_map_encoder() && s.m >= 16 && s.n >= 32 && s.k >= 32 && s.n <= (1 << 24) && s.k <= (1 << 24) &&
+         m * n <= most && m * k <= most && k * n <= most;
 }
 
 }  // namespace
 
 int nrs_tc_gated_fwd(nrs_ctx* ctx, const Shape& s, const float* x, const float* w_gate, const float* w_up, float* h, float* pre_gate, float* pre_up) {
   if (!applies(ctx, s)) return NRS_ERR_UNSUPPORTED;
-  Planes A{}, B{};
-  int st = stage_x(ctx, s, x, &A);
-  if (st == NRS_OK) st = stage_weights(ctx, s, w_gate, w_up, true, &B);
+  Planes X{}, W{};
+  int st = open_planes(ctx, NRS_WS_A, s.m, s.k, 1, &X);
+  if (st == NRS_OK) st = open_planes(ctx, NRS_WS_B, s.k, s.n, 2, &W);
+  if (st != NRS_OK) return st;
+  Jobs jobs{};
+  add_job(&jobs, x, nullptr, nullptr, s.m, s.k, X, 0);
+  add_job(&jobs, w_gate, nullptr, nullptr, s.k, s.n, W, 0);
+  add_job(&jobs, w_up, nullptr, nullptr, s.k, s.n, W, 1);
+  st = run_jobs<true>(ctx, jobs);
+  if (st == NRS_OK) st = run_jobs<false>(ctx, jobs);
   if (st != NRS_OK) return st;
   GatedPolicy<kForward> pol{};
   pol.out[0] = h; pol.pre[0] = pre_gate; pol.pre[1] = pre_up;
-  pol.M = s.m; pol.N = s.n; pol.act = s.act;
+  pol.M = s.m; pol.N = s.n; pol.ld = W.pad; pol.act = s.act;
   pol.vec = s.n % 4 == 0 && aligned({h, pre_gate, pre_up});
   NrsProfScope prof(ctx, NRS_PROF_GEMM, 4.0 * s.m * s.n * s.k);
-  const int ld = round64(s.k), cols = 2 * round64(s.n), kb = ld / 64;
   // Pairs take 395 clocks per 32 values of K a round of 74, single tiles 530 a round of 148 (plan_tile's table).
-  const long tm = (s.m + 127) / 128, tn = cols / 128, sms = ctx->sm_count;
+  const long tm = (s.m + 127) / 128, tn = W.pad / 64, sms = ctx->sm_count;
   const long pairs = ((tm + 1) / 2 * tn + sms / 2 - 1) / (sms / 2) * 395, singles = (tm * tn + sms - 1) / sms * 530;
-  if (pairs <= singles) return run<128, true, kForward>(ctx, A, B, pol, s.m, cols, s.k, 1, ld, (size_t)s.m * ld, s.n, ld, (size_t)s.n * ld, kb);
-  return run<128, false, kForward>(ctx, A, B, pol, s.m, cols, s.k, 1, ld, (size_t)s.m * ld, s.n, ld, (size_t)s.n * ld, kb);
+  return pairs <= singles ? run<128, true, kForward>(ctx, X, W, pol, s.m, W.ld, s.k) : run<128, false, kForward>(ctx, X, W, pol, s.m, W.ld, s.k);
 }
 
 int nrs_tc_gated_bwd(nrs_ctx* ctx, const Shape& s, const float* x, const float* w_gate, const float* w_up, const float* pre_gate, const float* pre_up,
                      const float* dh, float* dx, float* dw_gate, float* dw_up, int acc_x, int acc_w) {
   if (!applies(ctx, s)) return NRS_ERR_UNSUPPORTED;
-  const int ldn = round64(s.n), ldk = round64(s.k);
-  Planes D{};
-  int st = nrs_ws_planes(ctx, NRS_WS_GATED, 2 * (size_t)s.m * ldn, true, &D.hi, &D.lo);
+  Planes D{}, X{}, W{};
+  int st = open_planes(ctx, NRS_WS_GATED, s.m, s.n, 2, &D);
+  if (st == NRS_OK && dw_gate) st = open_planes(ctx, NRS_WS_A, s.m, s.k, 1, &X);
+  if (st == NRS_OK && dx) st = open_planes(ctx, NRS_WS_B, s.k, s.n, 2, &W);
   if (st != NRS_OK) return st;
-  NrsRange* range = nullptr;
-  st = nrs_range_renew(ctx, D.hi, &range);
-  if (st != NRS_OK) return st;
-  D.range = range;
-  const bool vec = s.n % 4 == 0 && aligned({dh, pre_gate, pre_up});
-  const uint32_t quads = (uint32_t)s.m * (uint32_t)(ldn / 4);
-  const unsigned blocks = std::min<unsigned>((quads + 511) / 512, (unsigned)ctx->sm_count * 8);
-  NRS_PDL_LAUNCH(gated_planes_kernel<false>, blocks, 256, 0, ctx->stream, dh, pre_gate, pre_up, (float*)D.hi, (float*)D.lo, range, s.m, s.n, ldn,
-                 NrsFastDiv(ldn / 4), s.act, vec);
-  NRS_LAUNCHED(ctx);
-  NRS_PDL_LAUNCH(gated_planes_kernel<true>, blocks, 256, 0, ctx->stream, dh, pre_gate, pre_up, (float*)D.hi, (float*)D.lo, range, s.m, s.n, ldn,
-                 NrsFastDiv(ldn / 4), s.act, vec);
-  NRS_LAUNCHED(ctx);
-  const size_t ld2 = 2 * (size_t)ldn;
+  Jobs jobs{};
+  jobs.act = s.act;
+  add_job(&jobs, dh, pre_gate, pre_up, s.m, s.n, D, 0);
+  if (dw_gate) add_job(&jobs, x, nullptr, nullptr, s.m, s.k, X, 0);
   if (dx) {
-    Planes W{};
-    st = stage_weights(ctx, s, w_gate, w_up, false, &W);
-    if (st != NRS_OK) return st;
+    add_job(&jobs, w_gate, nullptr, nullptr, s.k, s.n, W, 0);
+    add_job(&jobs, w_up, nullptr, nullptr, s.k, s.n, W, 1);
+  }
+  st = run_jobs<true>(ctx, jobs);
+  if (st == NRS_OK) st = run_jobs<false>(ctx, jobs);
+  if (st != NRS_OK) return st;
+  if (dx) {
     GatedPolicy<kInput> pol{};
-    pol.out[0] = dx; pol.M = s.m; pol.N = s.k; pol.ld = ldn; pol.accumulate = acc_x;
+    pol.out[0] = dx; pol.M = s.m; pol.N = s.k; pol.ld = D.pad; pol.accumulate = acc_x;
     pol.vec = s.k % 4 == 0 && aligned({dx});
     NrsProfScope prof(ctx, NRS_PROF_GEMM, 4.0 * s.m * s.n * s.k);
-    const tc::TilePlan t = tc::plan_tile(ctx, (s.m + 127) / 128, s.k, 1, 2 * ldn / 32, true, 0.004, false, false);
-#define NRS_RUN(BN_, PAIR_) run<BN_, PAIR_, kInput>(ctx, D, W, pol, s.m, s.k, s.n, 2, ld2, ldn, s.k, ldn, (size_t)s.k * ldn, 2 * ldn / 64)
+    const tc::TilePlan t = tc::plan_tile(ctx, (s.m + 127) / 128, s.k, 1, D.ld / 32, true, 0.004, false, false);
+#define NRS_RUN(BN_, PAIR_) run<BN_, PAIR_, kInput>(ctx, D, W, pol, s.m, s.k, s.n)
     st = t.bn == 128 ? (t.pair ? NRS_RUN(128, true) : NRS_RUN(128, false)) : (t.pair ? NRS_RUN(64, true) : NRS_RUN(64, false));
 #undef NRS_RUN
     if (st != NRS_OK) return st;
   }
-  if (dw_gate || dw_up) {
-    Planes X{};
-    st = stage_x(ctx, s, x, &X);
-    if (st != NRS_OK) return st;
+  if (dw_gate) {
     GatedPolicy<kWeights> pol{};
-    pol.out[0] = dw_gate; pol.out[1] = dw_up; pol.M = s.k; pol.N = s.n; pol.ld = ldn; pol.accumulate = acc_w;
+    pol.out[0] = dw_gate; pol.out[1] = dw_up; pol.M = s.k; pol.N = s.n; pol.ld = D.pad; pol.accumulate = acc_w;
     pol.vec = s.n % 4 == 0 && aligned({dw_gate, dw_up});
     NrsProfScope prof(ctx, NRS_PROF_GEMM, 4.0 * s.m * s.n * s.k);
-    const tc::TilePlan t = tc::plan_tile(ctx, (s.k + 127) / 128, 2 * ldn, 1, (s.m + 31) / 32, true, 0.004, false, false);
-#define NRS_RUN(BN_, PAIR_) run<BN_, PAIR_, kWeights>(ctx, X, D, pol, s.k, 2 * ldn, s.m, 1, ldk, 0, 0, ld2, 0, (s.m + 63) / 64)
+    const tc::TilePlan t = tc::plan_tile(ctx, (s.k + 127) / 128, D.ld, 1, (s.m + 31) / 32, true, 0.004, false, false);
+#define NRS_RUN(BN_, PAIR_) run<BN_, PAIR_, kWeights>(ctx, X, D, pol, s.k, D.ld, s.m)
     // (columns of 64 in a CTA's share of B: no pair of 64)
     st = t.bn == 128 && t.pair ? NRS_RUN(128, true) : t.bn == 128 ? NRS_RUN(128, false) : NRS_RUN(64, false);
 #undef NRS_RUN
-    if (st != NRS_OK) return st;
   }
-  return NRS_OK;
+  return st;
 }

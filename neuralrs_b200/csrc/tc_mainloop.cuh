@@ -221,6 +221,45 @@ __device__ __forceinline__ void rows_to_lines(float* tile, int lane, const uint3
   for (int i = 0; i < 4; ++i) v[i] = t4[chunk(8 * i + (lane >> 2), lane & 3)];
 }
 
+// The same 32 x 16 values to rows of a matrix, `rows` and `cols` of which exist; `add`: to what is there.  VEC: whole columns
+// of four, on 16 bytes.  Otherwise a store covers two rows of 64 bytes, value by value (four neighbours a lane, as above,
+// would touch eight rows in pieces of 16 bytes four times over).
+template <bool VEC>
+__device__ __forceinline__ void block_to_rows(float* tile, int lane, const float (&s)[16], float* dst, size_t ld, int rows, int cols, bool add) {
+  uint32_t r[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(s[j]);
+  float4 v[4];
+  rows_to_lines(tile, lane, r, v);   // (and leaves them in the tile)
+  if (VEC) {
+    const int c = (lane & 3) * 4;
+    if (c >= cols) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 8 * i + (lane >> 2);
+      if (row >= rows) return;
+      float4* p = reinterpret_cast<float4*>(dst + (size_t)row * ld + c);
+      if (add) {
+        const float4 o = *p;
+        v[i] = make_float4(o.x + v[i].x, o.y + v[i].y, o.z + v[i].z, o.w + v[i].w);
+      }
+      *p = v[i];
+    }
+  } else {
+    const int c = lane & 15;
+    if (c < cols) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int row = 2 * i + (lane >> 4);
+        if (row >= rows) break;
+        float* p = dst + (size_t)row * ld + c;
+        const float x = tile[(row * 4 + ((c >> 2) ^ ((row >> 1) & 3))) * 4 + (c & 3)];
+        *p = add ? *p + x : x;
+      }
+    }
+  }
+}
+
 // The column blocks of an epilogue warp: block c of a tile is its columns [c * kW, (c + 1) * kW); a warp takes c_first,
 // c_first + kStep, ...
 template <int BN, class Policy>
@@ -594,25 +633,26 @@ tc_kernel(const __grid_constant__ CUtensorMap tm_a_hi, const __grid_constant__ C
         if (!ok) break;
         if (!takes_part) continue;
         float* scratch = reinterpret_cast<float*>(emit_tile) + (warp - 2) * 512;
-        const int r0 = q * 32 + (lane >> 2);
+        const int m0 = tile_m * BM + q * 32;
         if constexpr (Policy::kGated) {
-          pol.template finish<kMine>(tile_m, tile_n, c_first, r0, lane, scratch, sums, top);
+          pol.template finish<kMine>(m0, tile_n, c_first, lane, scratch, sums);
         } else {
 #pragma unroll
           for (int i = 0; i < kMine; ++i) {
-            const int c = c_first + i * kStep, n = n0 + c * kW + (lane & 3) * 4;
-            if (n0 + c * kW >= sp.n_total) continue;
-            uint32_t r[kW];
-#pragma unroll
-            for (int j = 0; j < kW; ++j) r[j] = __float_as_uint(sums[i][j]);
-            float4 v[4];
-            rows_to_lines(scratch, lane, r, v);
+            const int n = n0 + (c_first + i * kStep) * kW;
+            if (n >= sp.n_total) continue;
             if (sp.splits > 1) {
-              float* dst = sp.partial + (((size_t)split * sp.batches + batch) * sp.rows_total + (size_t)tile_m * BM + r0) * sp.n_total + n;
+              uint32_t r[kW];
 #pragma unroll
-              for (int j = 0; j < 4; ++j, dst += (size_t)8 * sp.n_total) store_guarded(dst, v[j], sp.n_total - n, sp.n_total % 4 == 0);
+              for (int j = 0; j < kW; ++j) r[j] = __float_as_uint(sums[i][j]);
+              float4 v[4];
+              rows_to_lines(scratch, lane, r, v);
+              const int at = n + (lane & 3) * 4;
+              float* dst = sp.partial + (((size_t)split * sp.batches + batch) * sp.rows_total + m0 + (lane >> 2)) * sp.n_total + at;
+#pragma unroll
+              for (int j = 0; j < 4; ++j, dst += (size_t)8 * sp.n_total) store_guarded(dst, v[j], sp.n_total - at, sp.n_total % 4 == 0);
             } else {
-              pol.epilogue(tile_m, r0, n, v);
+              pol.block(m0, n, lane, scratch, sums[i]);
             }
           }
         }
