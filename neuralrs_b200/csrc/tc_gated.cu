@@ -36,6 +36,7 @@ struct GatedPolicy {
   int ld;                // n, padded: columns of one of the two matrices side by side
   int act, accumulate;
   bool vec;              // rows of the outputs start on 16 bytes
+  bool independent;      // of the kernel launched before it
 
   __device__ __forceinline__ bool clip(int, int, int, int*, int*) const { return true; }
   __device__ __forceinline__ uint32_t a_slice_rows() const { return tc::BM; }
@@ -99,15 +100,43 @@ struct GatedPolicy {
     if (c >= N) return;
     send(out[mat] + (size_t)m0 * N + c, m0, c, lane, scratch, v);
   }
-  // One element, from the pass that sums a K-split.
-  template <bool SPLIT>
-  __device__ __forceinline__ void store(int tile_m, int, int row, int n, float v, float, uint32_t&) const {
-    const int mat = P == kWeights && n >= ld ? 1 : 0, c = n - mat * ld, m = tile_m * tc::BM + row;
-    if (m >= M || c >= N) return;
-    float* dst = out[mat] + (size_t)m * N + c;
-    *dst = accumulate ? *dst + v : v;
-  }
+  int sum_splits(nrs_ctx* ctx, const tc::SplitInfo& sp) const;
 };
+
+// The splits' partial products, four columns a thread, added up in order.  (8 MB of them in 2.5 us where a value a thread,
+// its place found by two 64-bit divisions, took 7.)
+template <Product P>
+__global__ void __launch_bounds__(256) gated_splits_kernel(const GatedPolicy<P> pol, const tc::SplitInfo sp, NrsFastDiv div /*of quads*/) {
+  NRS_PDL_PROLOGUE();
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  uint32_t row, q;
+  div.divmod(i, row, q);
+  if ((int)row >= pol.M) return;
+  const int n = 4 * (int)q, mat = P == kWeights && n >= pol.ld ? 1 : 0, c = n - mat * pol.ld;
+  const bool whole = sp.n_total % 4 == 0;
+  const size_t per = (size_t)sp.rows_total * sp.n_total;
+  const float* src = sp.partial + (size_t)row * sp.n_total + n;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int z = 0; z < sp.splits; ++z) {
+    const float4 o = tc::load_guarded(src + z * per, sp.n_total - n, whole);
+    v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+  }
+  if (c >= pol.N) return;
+  float* dst = pol.out[mat] + (size_t)row * pol.N + c;
+  if (pol.accumulate) {
+    const float4 o = tc::load_guarded(dst, pol.N - c, pol.vec);
+    v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+  }
+  tc::store_guarded(dst, v, pol.N - c, pol.vec);
+}
+template <Product P>
+int GatedPolicy<P>::sum_splits(nrs_ctx* ctx, const tc::SplitInfo& sp) const {
+  const uint32_t quads = (uint32_t)(sp.n_total + 3) / 4;   // (a split product is at most half a wave of tiles)
+  NRS_PDL_LAUNCH(gated_splits_kernel<P>, ((uint32_t)M * quads + 255) / 256, 256, 0, ctx->stream, *this, sp, NrsFastDiv((int)quads));
+  NRS_LAUNCHED(ctx);
+  return NRS_OK;
+}
 
 // ------------------------------------------------------------------------------------------------ operand planes
 
@@ -149,7 +178,7 @@ __device__ __forceinline__ void put8(__half* hi, __half* lo, size_t at, const fl
 // slope exceeds, and of dh a, which no activation exceeds; without their exponentials this is a pass at memory speed.
 // Otherwise the pairs, zeros from cols to pad.
 template <bool MEASURE>
-__global__ void __launch_bounds__(256) gated_stage_kernel(const Jobs jobs) {
+__global__ void __launch_bounds__(256, MEASURE ? 3 : 4) gated_stage_kernel(const Jobs jobs) {
   NRS_PDL_PROLOGUE();
   int which = 0;
   while (which + 1 < jobs.count && blockIdx.x >= jobs.j[which + 1].first) ++which;
@@ -159,7 +188,7 @@ __global__ void __launch_bounds__(256) gated_stage_kernel(const Jobs jobs) {
   const float bound = MEASURE ? 0.0f : q.range->top, scale = MEASURE ? 1.0f : pr::scale_of(bound);
   if (!MEASURE && blockIdx.x == q.first && threadIdx.x == 0) q.range->bound = bound;
   uint32_t top = 0;
-  constexpr int kDeep = 2;
+  constexpr int kDeep = MEASURE ? 2 : 1;
   for (uint32_t i0 = (blockIdx.x - q.first) * 256 + threadIdx.x; i0 < units; i0 += kDeep * step) {
     float g[kDeep][8], a[kDeep][8], u[kDeep][8];
     uint32_t row[kDeep], col[kDeep];
@@ -208,9 +237,12 @@ __global__ void __launch_bounds__(256) gated_stage_kernel(const Jobs jobs) {
       }
     }
   }
-  if (MEASURE) {
-    __syncwarp();
-    pr::report(q.range, top);
+  if (MEASURE) {   // (one atomic a block: those of ten thousand warps on one word took longer than the pass)
+    __shared__ uint32_t tops[8];
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x < 32) pr::report(q.range, threadIdx.x < 8 ? tops[threadIdx.x] : 0u);
   }
 }
 
@@ -274,7 +306,7 @@ bool map_mn(CUtensorMap* t, const void* base, const Planes& p, int k, int box_co
 
 // The product of A [rows] and B [cols, padding included]; k: its length (input: of one matrix).
 template <int BN, bool PAIR, Product P>
-int run(nrs_ctx* ctx, const Planes& A, const Planes& B, const GatedPolicy<P>& pol, int rows, int cols, int k) {
+int run(nrs_ctx* ctx, const Planes& A, const Planes& B, const GatedPolicy<P>& pol, int rows, int cols, int k, int* splits = nullptr) {
   constexpr int kBCols = PAIR || P == kForward ? BN / 2 : BN;   // of B in one load
   CUtensorMap a[2], b[2];
   bool ok = true;
@@ -286,7 +318,7 @@ int run(nrs_ctx* ctx, const Planes& A, const Planes& B, const GatedPolicy<P>& po
   NRS_REQUIRE(ctx, ok, NRS_ERR_CUDA, "gated layer: cuTensorMapEncodeTiled failed (%d x %d x %d)", rows, cols, k);
   const int kb = P == kInput ? 2 * (A.pad / 64) : (k + 63) / 64;
   return tc::launch<BN, 2, PAIR, 64, GatedPolicy<P>>(ctx, a[0], a[1], b[0], b[1], pol, (rows + tc::BM - 1) / tc::BM, cols, 1, kb,
-                                                     tc::Ranges{A.range, B.range, nullptr});
+                                                     tc::Ranges{A.range, B.range, nullptr}, nullptr, nullptr, splits);
 }
 
 bool applies(const nrs_ctx* ctx, const Shape& s) {
@@ -341,13 +373,14 @@ int nrs_tc_gated_bwd(nrs_ctx* ctx, const Shape& s, const float* x, const float* 
   st = run_jobs<true>(ctx, jobs);
   if (st == NRS_OK) st = run_jobs<false>(ctx, jobs);
   if (st != NRS_OK) return st;
+  int splits = 0;   // of the product for dx (0: there is none)
   if (dx) {
     GatedPolicy<kInput> pol{};
     pol.out[0] = dx; pol.M = s.m; pol.N = s.k; pol.ld = D.pad; pol.accumulate = acc_x;
     pol.vec = s.k % 4 == 0 && aligned({dx});
     NrsProfScope prof(ctx, NRS_PROF_GEMM, 4.0 * s.m * s.n * s.k);
     const tc::TilePlan t = tc::plan_tile(ctx, (s.m + 127) / 128, s.k, 1, D.ld / 32, true, 0.004, false, false);
-#define NRS_RUN(BN_, PAIR_) run<BN_, PAIR_, kInput>(ctx, D, W, pol, s.m, s.k, s.n)
+#define NRS_RUN(BN_, PAIR_) run<BN_, PAIR_, kInput>(ctx, D, W, pol, s.m, s.k, s.n, &splits)
     st = t.bn == 128 ? (t.pair ? NRS_RUN(128, true) : NRS_RUN(128, false)) : (t.pair ? NRS_RUN(64, true) : NRS_RUN(64, false));
 #undef NRS_RUN
     if (st != NRS_OK) return st;
@@ -356,6 +389,9 @@ int nrs_tc_gated_bwd(nrs_ctx* ctx, const Shape& s, const float* x, const float* 
     GatedPolicy<kWeights> pol{};
     pol.out[0] = dw_gate; pol.out[1] = dw_up; pol.M = s.k; pol.N = s.n; pol.ld = D.pad; pol.accumulate = acc_w;
     pol.vec = s.n % 4 == 0 && aligned({dw_gate, dw_up});
+    // It reads nothing that the product for dx wrote, and starts on the SMs that one leaves idle; but not over partial sums
+    // that are still being added up.
+    pol.independent = splits == 1;
     NrsProfScope prof(ctx, NRS_PROF_GEMM, 4.0 * s.m * s.n * s.k);
     const tc::TilePlan t = tc::plan_tile(ctx, (s.k + 127) / 128, D.ld, 1, (s.m + 31) / 32, true, 0.004, false, false);
 #define NRS_RUN(BN_, PAIR_) run<BN_, PAIR_, kWeights>(ctx, X, D, pol, s.k, D.ld, s.m)

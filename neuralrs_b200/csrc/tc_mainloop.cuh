@@ -320,7 +320,12 @@ tc_kernel(const __grid_constant__ CUtensorMap tm_a_hi, const __grid_constant__ C
   const uint32_t tmem_base = uniform(*tmem_slot);
   // Everything above (barriers, tensor memory, descriptor prefetch) may overlap the tail of the kernel
   // before this one in the stream; from here on its results are needed.
-  NRS_PDL_WAIT();
+  // (A product marked independent of that kernel waits before it ends instead: see NRS_PDL_PROLOGUE.)
+  if constexpr (ShortChains<Policy>::value) {
+    if (!pol.independent) NRS_PDL_WAIT();
+  } else {
+    NRS_PDL_WAIT();
+  }
   NRS_PDL_TRIGGER();   // the next kernel may be scheduled as this grid's SMs free up
 
   if constexpr (Policy::kSlab) {
@@ -802,6 +807,9 @@ tc_kernel(const __grid_constant__ CUtensorMap tm_a_hi, const __grid_constant__ C
     if (emit_issuer) bulk_wait_all();   // shared memory must outlive the stores that read it
   }
 
+  if constexpr (ShortChains<Policy>::value) {
+    if (pol.independent) NRS_PDL_WAIT();
+  }
   tc_fence_before_sync();
   // (a pair: neither CTA may leave while the other's UMMAs read its memory or arrive on its barriers)
   __syncwarp();
@@ -982,7 +990,9 @@ int launch(nrs_ctx* ctx, const CUtensorMap& ta_hi, const CUtensorMap& ta_lo, con
   (void)nrs_pdl_launch_cluster(PAIR ? 2 : 1, tc_kernel<BN, NPLANES, Policy, PAIR, KW>, dim3(grid), dim3(threads<Policy>()), (size_t)kSmem, ctx->stream,
                                ta_hi, ta_lo, tb_hi, tb_lo, out_hi ? *out_hi : ta_hi, out_lo ? *out_lo : ta_hi, pol, sp, tmap, emit, rg, err);
   NRS_LAUNCHED(ctx);
-  if (sp.splits > 1) {
+  if constexpr (ShortChains<Policy>::value) {
+    if (sp.splits > 1) return pol.sum_splits(ctx, sp);
+  } else if (sp.splits > 1) {
     const size_t per = (size_t)batches * sp.rows_total * n_total;
     NRS_PDL_LAUNCH((tc_splitk_reduce_kernel<NPLANES == 2, Policy>), nrs_blocks(per, 256), 256, 0, ctx->stream, pol, sp, rg.out);
     NRS_LAUNCHED(ctx);
