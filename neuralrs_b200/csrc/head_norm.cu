@@ -11,11 +11,16 @@
 // Bound by memory: 8 bytes a feature forward, 12 backward.  A row is held in the registers of L neighbouring lanes, eight
 // features each in two 16-byte accesses, placed so that a lane holds both members of its pairs: nothing but the row sum
 // crosses lanes.  A warp works on one token at a time: the angles are looked up once for all its heads.
+#include <algorithm>
+
+#include "igemm_problems.cuh"
 #include "nrs_internal.h"
 
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kDeep = 2;                            // rows of a lane under way together
+constexpr int kBlocksFwd = 3, kBlocksBwd = 2;       // blocks an SM, all of them resident
 constexpr int kErrBadPosition = 6;
 constexpr int kMaxHead = 1024;
 
@@ -26,15 +31,17 @@ struct Side {   // of the queries, or of the keys
   float* y;             // forward: the result; backward: dx, or null
   float* partial;       // backward: [blocks of this side][d], or null
   long ld_x, ld_g, ld_y;
-  int heads, chunks;    // a warp's task: one token, heads [chunk * per, (chunk + 1) * per)
+  int heads;
   int first_block, blocks;
+  NrsFastDiv div;       // of heads
 };
 struct Args {
   Side side[2];
   const float* table;     // [max_len][rot / 2][cos, sin], or null
   const int32_t* pos;     // or null: t % seq
   int* err;
-  int tokens, seq, d, rot, max_len, per, accumulate;
+  int tokens, seq, d, rot, max_len, accumulate;
+  NrsFastDiv div_seq;
   float eps, inv_d;
 };
 
@@ -43,7 +50,14 @@ __device__ __forceinline__ int token_of(long i, int per) { return i >> 32 ? (int
 // The position of token t, or -1 outside the table.
 __device__ __forceinline__ int position(const Args& a, int t) {
   if (!a.table) return 0;
-  const int p = a.pos ? a.pos[t] : t % a.seq;
+  int p;
+  if (a.pos) {
+    p = a.pos[t];
+  } else {
+    uint32_t q, r;
+    a.div_seq.divmod((uint32_t)t, q, r);
+    p = (int)r;
+  }
   return p >= 0 && p < a.max_len ? p : -1;
 }
 
@@ -85,12 +99,13 @@ __device__ __forceinline__ void get(float (&v)[4], const float* p, bool on) {
 }
 __device__ __forceinline__ void put(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 
-// L: lanes of a row.  d and rot are multiples of 8, d <= 8 * L, every row starts on 16 bytes.
+// L: lanes of a row.  d and rot are multiples of 8, d <= 8 * L, every row starts on 16 bytes.  A row is a token's head; a warp
+// takes 32 / L of them side by side and kDeep times that together, so that their loads, and behind the positions those of the
+// table, are all under way before the first sum.
 template <int L, bool INTER, bool BWD>
-__global__ void __launch_bounds__(kThreads) head_norm_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, BWD ? kBlocksBwd : kBlocksFwd) head_norm_kernel(const Args a) {
   NRS_PDL_PROLOGUE();
-  constexpr int R = 32 / L;           // rows of a warp at a time
-  constexpr int kDeep = BWD ? 2 : 4;  // ... and how many times that under way together
+  constexpr int R = 32 / L;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, u = lane % L, sub = lane / L;
   const bool keys = (int)blockIdx.x >= a.side[1].first_block;
   const Side& s = a.side[keys ? 1 : 0];
@@ -105,84 +120,88 @@ __global__ void __launch_bounds__(kThreads) head_norm_kernel(const Args a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) wa[j] = wb[j] = 1.0f;
   }
-  const long tasks = (long)a.tokens * s.chunks, step = (long)s.blocks * kWarps;
-  for (long task = (long)((int)blockIdx.x - s.first_block) * kWarps + warp; task < tasks; task += step) {
-    const int t = token_of(task, s.chunks), h0 = (int)(task - (long)t * s.chunks) * a.per, h1 = min(s.heads, h0 + a.per);
-    const int p = position(a, t);
-    if (p < 0 && lane == 0) atomicExch(a.err, kErrBadPosition);
-    float4 t0 = make_float4(1.0f, 0.0f, 1.0f, 0.0f), t1 = t0;
-    if (turns && p >= 0) {
-      const float* row = a.table + (size_t)p * a.rot;
-      t0 = *reinterpret_cast<const float4*>(row + ta);
-      t1 = *reinterpret_cast<const float4*>(row + tb);
-    }
-    const float* x = s.x + (size_t)t * s.ld_x;
-    const float* g = BWD ? s.g + (size_t)t * s.ld_g : nullptr;
-    float* y = s.y ? s.y + (size_t)t * s.ld_y : nullptr;
-    for (int h = h0 + sub; h < h1 + sub; h += R * kDeep) {   // (all lanes of a warp take the same rounds)
-      float A[kDeep][4], B[kDeep][4], GA[BWD ? kDeep : 1][4], GB[BWD ? kDeep : 1][4];
+  const uint32_t rows = (uint32_t)a.tokens * (uint32_t)s.heads, step = (uint32_t)s.blocks * (kWarps * R * kDeep);   // (the launcher checks the range)
+  for (uint32_t r0 = ((uint32_t)((int)blockIdx.x - s.first_block) * kWarps + warp) * (R * kDeep); r0 < rows; r0 += step) {
+    float A[kDeep][4], B[kDeep][4], GA[BWD ? kDeep : 1][4], GB[BWD ? kDeep : 1][4];
+    float4 t0[kDeep], t1[kDeep];
+    uint32_t t[kDeep], h[kDeep];
+    int p[kDeep];
 #pragma unroll
-      for (int k = 0; k < kDeep; ++k) {
-        const int hh = h + k * R;
-        const bool on = have && hh < h1;
-        get(A[k], x + (size_t)hh * a.d + oa, on);
-        get(B[k], x + (size_t)hh * a.d + ob, on);
-        if (BWD) {
-          get(GA[BWD ? k : 0], g + (size_t)hh * a.d + oa, on);
-          get(GB[BWD ? k : 0], g + (size_t)hh * a.d + ob, on);
-        }
+    for (int k = 0; k < kDeep; ++k) {
+      const uint32_t r = r0 + k * R + sub;
+      s.div.divmod(min(r, rows - 1), t[k], h[k]);
+      const bool on = have && r < rows;
+      const float* x = s.x + (size_t)t[k] * s.ld_x + h[k] * a.d;
+      get(A[k], x + oa, on);
+      get(B[k], x + ob, on);
+      if (BWD) {
+        const float* g = s.g + (size_t)t[k] * s.ld_g + h[k] * a.d;
+        get(GA[BWD ? k : 0], g + oa, on);
+        get(GB[BWD ? k : 0], g + ob, on);
       }
+    }
 #pragma unroll
-      for (int k = 0; k < kDeep; ++k) {
-        const int hh = h + k * R;
-        const bool on = have && hh < h1;
-        float sq = 0.0f;
+    for (int k = 0; k < kDeep; ++k) {
+      p[k] = position(a, t[k]);
+      t0[k] = t1[k] = make_float4(1.0f, 0.0f, 1.0f, 0.0f);
+      if (turns && p[k] >= 0) {
+        const float* row = a.table + (size_t)p[k] * a.rot;
+        t0[k] = *reinterpret_cast<const float4*>(row + ta);
+        t1[k] = *reinterpret_cast<const float4*>(row + tb);
+      }
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sq += A[k][j] * A[k][j] + B[k][j] * B[k][j];
-        const float rstd = rsqrtf(row_sum<L>(sq) * a.inv_d + a.eps);
-        if (!BWD) {
+    for (int k = 0; k < kDeep; ++k) {
+      const uint32_t r = r0 + k * R + sub;
+      const bool on = have && r < rows;
+      if (p[k] < 0 && u == 0 && r < rows) atomicExch(a.err, kErrBadPosition);
+      float sq = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) { A[k][j] *= rstd * wa[j]; B[k][j] *= rstd * wb[j]; }
-          if (turns) rotate<INTER>(A[k], B[k], t0, t1, false);
-          if (p < 0) {
+      for (int j = 0; j < 4; ++j) sq += A[k][j] * A[k][j] + B[k][j] * B[k][j];
+      const float rstd = rsqrtf(row_sum<L>(sq) * a.inv_d + a.eps);
+      if (!BWD) {
+        float* y = s.y + (size_t)t[k] * s.ld_y + h[k] * a.d;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) A[k][j] = B[k][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) { A[k][j] *= rstd * wa[j]; B[k][j] *= rstd * wb[j]; }
+        if (turns) rotate<INTER>(A[k], B[k], t0[k], t1[k], false);
+        if (p[k] < 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) A[k][j] = B[k][j] = 0.0f;
+        }
+        if (on) { put(y + oa, A[k]); put(y + ob, B[k]); }
+      } else {
+        float(&ga)[4] = GA[BWD ? k : 0];
+        float(&gb)[4] = GB[BWD ? k : 0];
+        if (p[k] < 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ga[j] = gb[j] = 0.0f;
+        }
+        if (turns) rotate<INTER>(ga, gb, t0[k], t1[k], true);
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          A[k][j] *= rstd; B[k][j] *= rstd;                       // the normed values
+          da[j] += ga[j] * A[k][j]; db[j] += gb[j] * B[k][j];
+          ga[j] *= wa[j]; gb[j] *= wb[j];
+          dot += ga[j] * A[k][j] + gb[j] * B[k][j];
+        }
+        const float mean = row_sum<L>(dot) * a.inv_d;
+        if (on && s.y) {
+          float* y = s.y + (size_t)t[k] * s.ld_y + h[k] * a.d;
+          float ra[4], rb[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { ra[j] = rstd * (ga[j] - A[k][j] * mean); rb[j] = rstd * (gb[j] - B[k][j] * mean); }
+          if (a.accumulate) {
+            float o[4];
+            get(o, y + oa, true);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ra[j] += o[j];
+            get(o, y + ob, true);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) rb[j] += o[j];
           }
-          if (on) { put(y + (size_t)hh * a.d + oa, A[k]); put(y + (size_t)hh * a.d + ob, B[k]); }
-        } else {
-          float(&ga)[4] = GA[BWD ? k : 0];
-          float(&gb)[4] = GB[BWD ? k : 0];
-          if (p < 0) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ga[j] = gb[j] = 0.0f;
-          }
-          if (turns) rotate<INTER>(ga, gb, t0, t1, true);
-          float dot = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            A[k][j] *= rstd; B[k][j] *= rstd;                       // the normed values
-            da[j] += ga[j] * A[k][j]; db[j] += gb[j] * B[k][j];
-            ga[j] *= wa[j]; gb[j] *= wb[j];
-            dot += ga[j] * A[k][j] + gb[j] * B[k][j];
-          }
-          const float mean = row_sum<L>(dot) * a.inv_d;
-          if (on && y) {
-            float ra[4], rb[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { ra[j] = rstd * (ga[j] - A[k][j] * mean); rb[j] = rstd * (gb[j] - B[k][j] * mean); }
-            float *pa = y + (size_t)hh * a.d + oa, *pb = y + (size_t)hh * a.d + ob;
-            if (a.accumulate) {
-              float o[4];
-              get(o, pa, true);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) ra[j] += o[j];
-              get(o, pb, true);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) rb[j] += o[j];
-            }
-            put(pa, ra);
-            put(pb, rb);
-          }
+          put(y + oa, ra);
+          put(y + ob, rb);
         }
       }
     }
@@ -326,18 +345,20 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(float* __restrict__ t
   }
 }
 
-// Blocks of the two sides: enough warps for the tasks, at most kBlocks blocks together, shared out by the sides' work.
-constexpr int kBlocksPerSm = 4;
-void plan_blocks(const nrs_ctx* ctx, Args* a, const long (&tasks)[2]) {
-  const long cap = (long)ctx->sm_count * kBlocksPerSm, all = tasks[0] + tasks[1];
-  int at = 0;
-  for (int i = 0; i < 2; ++i) {
-    const long want = (tasks[i] + kWarps - 1) / kWarps;
-    long most = cap;
-    if ((tasks[0] + kWarps - 1) / kWarps + (tasks[1] + kWarps - 1) / kWarps > cap) most = tasks[i] ? (cap * tasks[i] + all - 1) / all : 0;
+// Blocks of the two sides: enough for their rows, at most as many as are resident, shared out by the sides' rows.
+void plan_blocks(const nrs_ctx* ctx, Args* a, int per_block, int per_sm) {
+  const long cap = (long)ctx->sm_count * per_sm;
+  long want[2];
+  for (int i = 0; i < 2; ++i) want[i] = ((long)a->tokens * a->side[i].heads + per_block - 1) / per_block;
+  if (want[0] + want[1] > cap) {
+    long q = want[0] ? std::max(1L, cap * want[0] / (want[0] + want[1])) : 0;
+    if (want[1]) q = std::min(q, cap - 1);
+    want[1] = std::min(want[1], cap - q);
+    want[0] = q;
+  }
+  for (int i = 0, at = 0; i < 2; at += a->side[i++].blocks) {
     a->side[i].first_block = at;
-    a->side[i].blocks = (int)(want < most ? want : most);
-    at += a->side[i].blocks;
+    a->side[i].blocks = (int)want[i];
   }
 }
 
@@ -399,14 +420,12 @@ int launch(nrs_ctx* ctx, Args& a, const Shape& sh, float* workspace, int sums /*
     if (s.heads == 0) continue;
     vec = vec && (((uintptr_t)s.x | (uintptr_t)s.g | (uintptr_t)s.gamma | (uintptr_t)s.y) & 15) == 0 && s.ld_x % 4 == 0 && s.ld_g % 4 == 0 && s.ld_y % 4 == 0;
   }
-  long tasks[2];
-  const int round = (32 / lanes_of(a.d)) * (BWD ? 2 : 4);   // heads that a warp has under way together
-  a.per = round;
-  for (int i = 0; i < 2; ++i) {
-    a.side[i].chunks = (a.side[i].heads + a.per - 1) / a.per;
-    tasks[i] = (long)a.tokens * (vec ? a.side[i].chunks : a.side[i].heads);
+  for (Side& s : a.side) {
+    vec = vec && (long)a.tokens * s.heads <= 0x3fffffffL;
+    s.div = NrsFastDiv(s.heads > 0 ? s.heads : 1);
   }
-  plan_blocks(ctx, &a, tasks);
+  a.div_seq = NrsFastDiv(a.seq > 0 ? a.seq : 1);
+  plan_blocks(ctx, &a, vec ? kWarps * (32 / lanes_of(a.d)) * kDeep : kWarps, BWD ? kBlocksBwd : kBlocksFwd);
   const unsigned grid = (unsigned)(a.side[0].blocks + a.side[1].blocks);
   if (grid == 0) return NRS_OK;
   if (BWD) {
@@ -449,8 +468,8 @@ int nrs_qk_norm_rotary_fwd(nrs_ctx* ctx, const float* q, int64_t ld_q, const flo
   int st = check_shape(ctx, __func__, sh, table, positions);
   if (st != NRS_OK) return st;
   Args a{};
-  a.side[0] = Side{q, nullptr, gamma_q, q_out, nullptr, (long)ld_q, 0, (long)ld_q_out, heads_q, 0, 0, 0};
-  a.side[1] = Side{k, nullptr, gamma_k, k_out, nullptr, (long)ld_k, 0, (long)ld_k_out, heads_k, 0, 0, 0};
+  a.side[0] = Side{q, nullptr, gamma_q, q_out, nullptr, (long)ld_q, 0, (long)ld_q_out, heads_q, 0, 0, {}};
+  a.side[1] = Side{k, nullptr, gamma_k, k_out, nullptr, (long)ld_k, 0, (long)ld_k_out, heads_k, 0, 0, {}};
   if (tokens == 0) return NRS_OK;
   st = check_side(ctx, __func__, "queries", a.side[0], d_head, false);
   if (st == NRS_OK) st = check_side(ctx, __func__, "keys", a.side[1], d_head, false);
@@ -462,10 +481,10 @@ int nrs_qk_norm_rotary_fwd(nrs_ctx* ctx, const float* q, int64_t ld_q, const flo
   return launch<false>(ctx, a, sh, nullptr, 0);
 }
 
-// (Partial rows of d_head sums: one a block, of which there are as many as the rows fill and at most kBlocksPerSm an SM.)
+// (Partial rows of d_head sums: one a block, of which there are as many as the rows fill and at most kBlocksBwd an SM.)
 size_t nrs_qk_norm_rotary_workspace(int tokens, int heads_q, int heads_k, int d_head) {
   if (tokens <= 0 || heads_q < 0 || heads_k < 0 || d_head <= 0) return 0;
-  constexpr long kMost = 256L * kBlocksPerSm + 2;
+  constexpr long kMost = 256L * kBlocksBwd + 2;
   const long rows = (long)tokens * ((long)heads_q + heads_k) / kWarps + 2;
   return (size_t)(rows < kMost ? rows : kMost) * d_head * sizeof(float);
 }
@@ -480,8 +499,8 @@ int nrs_qk_norm_rotary_bwd(nrs_ctx* ctx, const float* g_q, int64_t ld_gq, const 
   int st = check_shape(ctx, __func__, sh, table, positions);
   if (st != NRS_OK) return st;
   Args a{};
-  a.side[0] = Side{q, g_q, gamma_q, dq, nullptr, (long)ld_q, (long)ld_gq, (long)ld_dq, heads_q, 0, 0, 0};
-  a.side[1] = Side{k, g_k, gamma_k, dk, nullptr, (long)ld_k, (long)ld_gk, (long)ld_dk, heads_k, 0, 0, 0};
+  a.side[0] = Side{q, g_q, gamma_q, dq, nullptr, (long)ld_q, (long)ld_gq, (long)ld_dq, heads_q, 0, 0, {}};
+  a.side[1] = Side{k, g_k, gamma_k, dk, nullptr, (long)ld_k, (long)ld_gk, (long)ld_dk, heads_k, 0, 0, {}};
   if (tokens > 0) {
     st = check_side(ctx, __func__, "queries", a.side[0], d_head, true);
     if (st == NRS_OK) st = check_side(ctx, __func__, "keys", a.side[1], d_head, true);
