@@ -8,6 +8,8 @@
 // a call is word i%4 of the block at counter (offset + i/4) under the context's 64-bit seed, u = (word >> 8) *
 // 2^-24 in [0,1), mask = u < p ? 0 : 1/(1-p).  The same seed and offset give the same mask on any launch
 // shape; a caller that wants the reference's own masks passes them to nrs_mask_mul instead.
+#include <cmath>
+
 #include "nrs_internal.h"
 #include "philox.cuh"
 
@@ -82,16 +84,28 @@ mask_mul_kernel(const float* __restrict__ a, const float* __restrict__ mask, flo
 // Dropout without a mask in memory: out = a * m (+ residual), or out (+)= a * m, with the mask of dropout_mask_kernel made
 // again wherever it is needed.  What a stored mask costs, 4 bytes written and read again in both passes and kept between
 // them, is spent on twenty wide multiplications per block of four instead, which run under the loads.
+// u < p is asked of the word itself: u = (word >> 8) 2^-24, so it holds for words up to 2^8 ceil(2^24 p) - 1 (p = 0, where
+// none are, has a dropped value's factor 1 instead).
+// Bound by memory, with the generator close behind: it takes half of the issue slots at full memory rate.  67 M values, both
+// passes: 205 us with u made and compared as a float, 199 as an integer, 190 compared as it comes and with counters whose
+// upper half all threads of a launch share (a call that crosses 2^32 takes two launches), which spares two of twenty
+// products, 178 with the form without a second operand compiled apart (39 registers, six blocks an SM); 165 with a toy
+// generator in its place.  The copy rate allows 166.
 //   FOURS: hw == 1, a block's four words serve four neighbouring elements; otherwise element i takes mask value i / hw
 //   VEC:   16-byte accesses (FOURS: aligned tensors; planes: hw a multiple of 4 too, so that a vector has one mask value)
-template <bool FOURS, bool VEC>
+struct Draw {
+  uint64_t seed, first;
+  uint32_t last;           // words up to here are dropped ones
+  float dropped, kept;     // their factor, and the others'
+  __device__ __forceinline__ float factor(uint32_t word) const { return word <= last ? dropped : kept; }
+};
+template <bool FOURS, bool VEC, bool ADD>
 __global__ void __launch_bounds__(kThreads)
-dropout_kernel(const float* a, const float* residual, float* out, size_t total, size_t hw, float p, float scale, uint64_t seed, uint64_t first,
-               int accumulate) {
+dropout_kernel(const float* a, const float* residual, float* out, size_t total, size_t hw, const Draw draw, int accumulate) {
   NRS_PDL_PROLOGUE();
   constexpr int kUnroll = 4;   // vectors of a thread under way together
   const size_t groups = (FOURS || VEC) ? (total + 3) / 4 : total;
-  const float* add = accumulate ? out : residual;
+  const float* add = ADD ? (accumulate ? out : residual) : nullptr;
   for (size_t base = (size_t)blockIdx.x * (kThreads * kUnroll) + threadIdx.x; base < groups; base += (size_t)gridDim.x * (kThreads * kUnroll)) {
     float4 v[kUnroll], r[kUnroll];
 #pragma unroll
@@ -101,17 +115,17 @@ dropout_kernel(const float* a, const float* residual, float* out, size_t total, 
       if (b >= groups) continue;
       if (VEC && 4 * b + 4 <= total) {
         v[u] = reinterpret_cast<const float4*>(a)[b];
-        if (add) r[u] = reinterpret_cast<const float4*>(add)[b];
+        if (ADD) r[u] = reinterpret_cast<const float4*>(add)[b];
       } else if (FOURS) {
         float e[4] = {}, f[4] = {};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (4 * b + j < total) { e[j] = a[4 * b + j]; if (add) f[j] = add[4 * b + j]; }
+          if (4 * b + j < total) { e[j] = a[4 * b + j]; if (ADD) f[j] = add[4 * b + j]; }
         v[u] = make_float4(e[0], e[1], e[2], e[3]);
         r[u] = make_float4(f[0], f[1], f[2], f[3]);
       } else {
         v[u].x = a[b];
-        if (add) r[u].x = add[b];
+        if (ADD) r[u].x = add[b];
       }
     }
 #pragma unroll
@@ -121,17 +135,17 @@ dropout_kernel(const float* a, const float* residual, float* out, size_t total, 
       uint32_t w[4];
       float4 m;
       if (FOURS) {
-        nrs_rng::block(seed, first + b, w);
-        m = make_float4(mask_value(w[0], p, scale), mask_value(w[1], p, scale), mask_value(w[2], p, scale), mask_value(w[3], p, scale));
+        nrs_rng::block(draw.seed, (draw.first >> 32 << 32) | (uint32_t)((uint32_t)draw.first + (uint32_t)b), w);
+        m = make_float4(draw.factor(w[0]), draw.factor(w[1]), draw.factor(w[2]), draw.factor(w[3]));
       } else {
         const size_t at = VEC ? 4 * b : b, i = (at | hw) >> 32 ? at / hw : (size_t)((uint32_t)at / (uint32_t)hw);
-        nrs_rng::block(seed, first + i / 4, w);
+        nrs_rng::block(draw.seed, draw.first + i / 4, w);
         const uint32_t k = (uint32_t)i & 3u;
-        const float one = mask_value(k < 2 ? (k == 0 ? w[0] : w[1]) : (k == 2 ? w[2] : w[3]), p, scale);
+        const float one = draw.factor(k < 2 ? (k == 0 ? w[0] : w[1]) : (k == 2 ? w[2] : w[3]));
         m = make_float4(one, one, one, one);
       }
       float4 y = make_float4(v[u].x * m.x, v[u].y * m.y, v[u].z * m.z, v[u].w * m.w);
-      if (add) {   // rounded once, as mask_mul_kernel does (but for the rest of a length that is no multiple of four)
+      if (ADD) {   // rounded once, as mask_mul_kernel does (but for the rest of a length that is no multiple of four)
         if (VEC && 4 * b + 4 > total) y = make_float4(__fadd_rn(r[u].x, y.x), __fadd_rn(r[u].y, y.y), __fadd_rn(r[u].z, y.z), 0.0f);
         else y = make_float4(fmaf(v[u].x, m.x, r[u].x), fmaf(v[u].y, m.y, r[u].y), fmaf(v[u].z, m.z, r[u].z), fmaf(v[u].w, m.w, r[u].w));
       }
@@ -224,20 +238,41 @@ static int dropout_pass(nrs_ctx* ctx, const char* who, const float* a, const flo
   NRS_REQUIRE(ctx, a && out, NRS_ERR_ARG, "%s: null tensor", who);
   NRS_REQUIRE(ctx, total % (size_t)hw == 0, NRS_ERR_SHAPE, "%s: %zu elements are not whole planes of %d", who, total, hw);
   NrsDeviceGuard on(ctx);
-  const float scale = 1.0f / (1.0f - p);   // (p == 1: infinite and never used, as in nrs_dropout_mask)
+  const uint32_t below = (uint32_t)std::ceil(p * 16777216.0f);
+  Draw draw{seed, first, (below << 8) - 1u, 0.0f, 1.0f / (1.0f - p)};   // (p == 1: every word, and the infinite factor is never used)
+  if (below == 0) { draw.last = 0; draw.dropped = 1.0f; }
   const bool aligned = (((uintptr_t)a | (uintptr_t)out | (uintptr_t)residual) & 15) == 0;
-  const size_t groups = hw == 1 || (aligned && hw % 4 == 0) ? (total + 3) / 4 : total;
-  const size_t want = (groups + 4 * kThreads - 1) / (4 * kThreads), cap = (size_t)ctx->sm_count * 16;
-  const unsigned blocks = (unsigned)(want > cap ? cap : want);
-#define NRS_DROPOUT(FOURS_, VEC_)                                                                                                       \
-  NRS_PDL_LAUNCH((dropout_kernel<FOURS_, VEC_>), blocks, kThreads, 0, ctx->stream, a, residual, out, total, (size_t)hw, p, scale, seed, \
-                 first, accumulate)
-  if (hw == 1 && aligned) NRS_DROPOUT(true, true);
-  else if (hw == 1) NRS_DROPOUT(true, false);
-  else if (aligned && hw % 4 == 0) NRS_DROPOUT(false, true);
-  else NRS_DROPOUT(false, false);
+  while (total > 0) {
+    size_t part = total;
+    if (hw == 1) {   // up to where the counter's upper half changes
+      const uint64_t left = ((uint64_t)1 << 32) - (uint32_t)draw.first;
+      if ((total + 3) / 4 > left) part = (size_t)left * 4;
+    }
+    const size_t groups = hw == 1 || (aligned && hw % 4 == 0) ? (part + 3) / 4 : part;
+    const size_t want = (groups + 4 * kThreads - 1) / (4 * kThreads), cap = (size_t)ctx->sm_count * 16;
+    const unsigned blocks = (unsigned)(want > cap ? cap : want);
+#define NRS_DROPOUT(FOURS_, VEC_)                                                                                                                     \
+  if (accumulate || residual)                                                                                                                         \
+    NRS_PDL_LAUNCH((dropout_kernel<FOURS_, VEC_, true>), blocks, kThreads, 0, ctx->stream, a, residual, out, part, (size_t)hw, draw, accumulate);      \
+  else                                                                                                                                                \
+    NRS_PDL_LAUNCH((dropout_kernel<FOURS_, VEC_, false>), blocks, kThreads, 0, ctx->stream, a, residual, out, part, (size_t)hw, draw, accumulate)
+    if (hw == 1 && aligned) {
+      NRS_DROPOUT(true, true);
+    } else if (hw == 1) {
+      NRS_DROPOUT(true, false);
+    } else if (aligned && hw % 4 == 0) {
+      NRS_DROPOUT(false, true);
+    } else {
+      NRS_DROPOUT(false, false);
+    }
 #undef NRS_DROPOUT
-  NRS_LAUNCHED(ctx);
+    NRS_LAUNCHED(ctx);
+    total -= part;
+    draw.first += part / 4;   // (with a total left, a part is whole blocks)
+    a += part;
+    out += part;
+    if (residual) residual += part;
+  }
   return NRS_OK;
 }
 

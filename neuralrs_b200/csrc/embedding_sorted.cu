@@ -7,13 +7,16 @@
 // token's row with atomics (:23-30); the form in transformer.cu gives every vocabulary row a block that looks through all
 // tokens, vocab * tokens comparisons.  Here two launches do tokens' work alone:
 //
-//   sort   every block owns a range of the vocabulary.  It looks through all ids once (they stay in L2), counts those below
-//          its range, which is where its own tokens start in the sorted order, and lists its own in the order of t; a
-//          stable counting sort of the list by id then needs no other block.  It writes the sorted (id, token) pairs and
-//          where each row's run starts, and zeroes the rows of the gradient that no token has.
+//   sort   every block owns a range of the vocabulary and looks through all ids (they stay in L2), a stretch of them a warp.
+//          It counts those below its range, which is where its own start in the sorted order, and for each of its rows
+//          and each warp the tokens there; the counts' running sums are the places, and a second look puts the tokens
+//          there, (id, token) by (id, token).  No block needs another, and no warp waits for one, also not where one id
+//          makes up most of the tokens.
 //   sum    the sorted tokens are cut into equal pieces, so a token that makes up a tenth of the text costs no block more
 //          than its share.  A run inside one piece goes straight to its row; one that crosses pieces leaves partial sums,
-//          and the last of its blocks to finish adds them up, in order.
+//          and the last of its blocks to finish adds them up, in order.  Other blocks among these write zeros to the rows
+//          that no token has: the sums wait for memory much, zeros not at all.  (Zeros by the sorting blocks beside their
+//          sort starve its loads: 16384 tokens x 1024 over 50000 rows 43 us for that launch, 36 for zeros behind it.)
 //
 // Deterministic: every sum has one order, whatever the blocks' timing.  Bound by memory: g read once, dweight written once.
 #include <algorithm>
@@ -70,10 +73,10 @@ embed_scaled_kernel(const float* __restrict__ w, const int32_t* __restrict__ idx
 // ------------------------------------------------------------------------------------------------ sort
 
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kTile = 4 * kSortThreads;   // tokens of a step: four neighbouring ids a thread
-constexpr int kMaxRange = 8192;           // most vocabulary rows of a block
+constexpr int kMaxRange = 1024;           // most vocabulary rows of a block: a count for each of them and each warp is 128 KB
 constexpr int kSumWarps = 8;              // of a block that sums
 constexpr int kSlab = 128;                // its columns
+constexpr int kZeroRows = 64;             // vocabulary rows of a block that writes zeros
 constexpr int kFillBlocks = 592;          // four for each of 148 SMs: fewer and pieces are made smaller
 
 struct Plan {
@@ -120,107 +123,79 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {   // inclusive
   }
   return v;
 }
-__device__ __forceinline__ void four_ids(const int32_t* idx, int t, int tokens, bool quads, int (&id)[4]) {
-  if (quads && t + 4 <= tokens) {
-    const int4 q = *reinterpret_cast<const int4*>(idx + t);
-    id[0] = q.x; id[1] = q.y; id[2] = q.z; id[3] = q.w;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) id[k] = t + k < tokens ? idx[t + k] : -1;
-  }
-}
-
 __global__ void __launch_bounds__(kSortThreads, 1)
-embed_sort_kernel(const int32_t* __restrict__ idx, const Plan p, const Work w, float* __restrict__ dw /*null: rows without tokens stay*/, bool vec) {
+embed_sort_kernel(const int32_t* __restrict__ idx, const Plan p, const Work w) {
   NRS_PDL_PROLOGUE();
-  extern __shared__ int smem[];
-  int2* list = reinterpret_cast<int2*>(smem);      // [kTile] a step's own tokens, in order
-  int* next = smem + 2 * kTile;                    // [range] tokens of each row, then where its next one goes
-  __shared__ int s_warp[2][kSortWarps];
+  extern __shared__ int counts[];                  // [warp][range] tokens of each row in the warp's stretch, then where its next goes
+  __shared__ int s_below[kSortWarps], s_scan[kSortWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int lo = blockIdx.x * p.range, hi = min(p.vocab, lo + p.range), rows = hi - lo;
-  const bool quads = (reinterpret_cast<uintptr_t>(idx) & 15) == 0;
-  for (int i = tid; i < rows; i += kSortThreads) next[i] = 0;
+  int* const mine = counts + warp * p.range;
+  // A warp's tokens: a stretch of its own, so the warps go through them without waiting for each other.
+  const int stretch = (p.tokens + kSortWarps - 1) / kSortWarps;
+  const int begin = (int)min((long)p.tokens, (long)warp * stretch), stop = (int)min((long)p.tokens, (long)begin + stretch);
+  for (int r = lane; r < rows; r += 32) mine[r] = 0;
   for (long i = (long)blockIdx.x * kSortThreads + tid; i < (long)p.pieces * p.slabs; i += (long)gridDim.x * kSortThreads) w.tickets[i] = 0;
-  __syncthreads();
+  __syncwarp();
 
   // How many tokens each row has, and how many lie below the range.  (Ids outside the vocabulary are nobody's.)
+  constexpr int kDeep = 8;                         // loads under way together
   int below = 0;
-  for (int t0 = 0; t0 < p.tokens; t0 += kTile) {
-    int id[4];
-    four_ids(idx, t0 + 4 * tid, p.tokens, quads, id);
+  for (int t0 = begin + lane; t0 < stop; t0 += 32 * kDeep) {
+    int id[kDeep];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kDeep; ++k) id[k] = t0 + 32 * k < stop ? idx[t0 + 32 * k] : -1;
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
       below += id[k] >= 0 && id[k] < lo;
-      if (id[k] >= lo && id[k] < hi) atomicAdd(&next[id[k] - lo], 1);
+      if (id[k] >= lo && id[k] < hi) atomicAdd(&mine[id[k] - lo], 1);
     }
   }
   below = warp_sum(below);
-  if (lane == 0) s_warp[0][warp] = below;
+  if (lane == 0) s_below[warp] = below;
   __syncthreads();
-  const int first = warp_sum(s_warp[0][lane]);     // where the range starts in the sorted order
+  const int first = warp_sum(s_below[lane]);       // where the range starts in the sorted order
 
-  // Counts to starts: a stretch of rows a thread.
-  const int each = (rows + kSortThreads - 1) / kSortThreads, r0 = min(rows, tid * each), r1 = min(rows, r0 + each);
-  int sum = 0;
-  for (int r = r0; r < r1; ++r) sum += next[r];
-  const int incl = warp_scan(sum, lane);
-  if (lane == 31) s_warp[1][warp] = incl;
-  __syncthreads();
-  int run = first + warp_sum(lane < warp ? s_warp[1][lane] : 0) + incl - sum;
-  for (int r = r0; r < r1; ++r) {
-    const int c = next[r];
-    next[r] = w.start[lo + r] = run;
-    run += c;
-  }
-  if (hi == p.vocab && r1 == rows && (r0 < rows || tid == 0)) w.start[p.vocab] = run;
-  __syncthreads();
-  const int end = first + warp_sum(s_warp[1][lane]);
-
-  // Each own token behind those of its id that came before it.
-  if (end > first) {
-    for (int t0 = 0, step = 0; t0 < p.tokens; t0 += kTile, ++step) {
-      const int t = t0 + 4 * tid;
-      int id[4], mine = 0;
-      four_ids(idx, t, p.tokens, quads, id);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) mine += id[k] >= lo && id[k] < hi;
-      const int before = warp_scan(mine, lane);
-      __syncthreads();                             // the step before has read its counts and its list
-      if (lane == 31) s_warp[0][warp] = before;
-      __syncthreads();
-      const int h = s_warp[0][lane], found = warp_sum(h);
-      int at = warp_sum(lane < warp ? h : 0) + before - mine;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (id[k] >= lo && id[k] < hi) list[at++] = make_int2(id[k] - lo, t + k);
-      __syncthreads();
-      if (warp == 0) {
-        for (int i0 = 0; i0 < found; i0 += 32) {
-          const bool on = i0 + lane < found;
-          const int2 e = on ? list[i0 + lane] : make_int2(-1, 0);
-          const unsigned same = __match_any_sync(0xffffffffu, e.x);
-          const int rank = __popc(same & ((1u << lane) - 1u)), to = on ? next[e.x] + rank : 0;
-          __syncwarp();
-          if (on) {
-            w.sorted[to] = make_int2(e.x + lo, e.y);
-            if (rank == 0) next[e.x] = to + __popc(same);
-          }
-          __syncwarp();
-        }
-      }
+  // Counts to places: a row a thread, its warps' tokens behind each other, the rows likewise.
+  int total = 0;
+  if (tid < rows) {
+#pragma unroll 8
+    for (int k = 0; k < kSortWarps; ++k) {
+      const int c = counts[k * p.range + tid];
+      counts[k * p.range + tid] = total;
+      total += c;
     }
   }
-  if (!dw) return;
+  const int incl = warp_scan(total, lane);
+  if (lane == 31) s_scan[warp] = incl;
   __syncthreads();
-  // Rows without a token: `next` now holds where each ends.
-  for (int r = warp; r < rows; r += kSortWarps) {
-    if (next[r] != (r ? next[r - 1] : first)) continue;
-    float* row = dw + (size_t)(lo + r) * p.dim;
-    if (vec)
-      for (int c = lane; c < p.dim / 4; c += 32) reinterpret_cast<float4*>(row)[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    else
-      for (int c = lane; c < p.dim; c += 32) row[c] = 0.0f;
+  const int start = first + warp_sum(lane < warp ? s_scan[lane] : 0) + incl - total;
+  if (tid < rows) {
+    w.start[lo + tid] = start;
+#pragma unroll 8
+    for (int k = 0; k < kSortWarps; ++k) counts[k * p.range + tid] += start;
+  }
+  if (hi == p.vocab && tid == rows - 1) w.start[p.vocab] = start + total;
+  __syncthreads();
+
+  // Each token behind those of its id that came before it, 32 at a time.
+  for (int t0 = begin; t0 < stop; t0 += 32 * kDeep) {
+    int id[kDeep];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) id[k] = t0 + 32 * k + lane < stop ? idx[t0 + 32 * k + lane] : -1;
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const bool hit = id[k] >= lo && id[k] < hi;
+      if (!__any_sync(0xffffffffu, hit)) continue;
+      const unsigned same = __match_any_sync(0xffffffffu, hit ? id[k] : -1);
+      const int rank = __popc(same & ((1u << lane) - 1u)), to = hit ? mine[id[k] - lo] + rank : 0;
+      __syncwarp();
+      if (hit) {
+        w.sorted[to] = make_int2(id[k], t0 + 32 * k + lane);
+        if (rank == 0) mine[id[k] - lo] = to + __popc(same);
+      }
+      __syncwarp();
+    }
   }
 }
 
@@ -252,15 +227,35 @@ struct Cols {
 
 template <bool VEC>
 __global__ void __launch_bounds__(kSumWarps * 32)
-embed_sum_kernel(const float* __restrict__ g, const Plan p, const Work w, float* dw, float scale, int accumulate) {
+embed_sum_kernel(const float* __restrict__ g, const Plan p, const Work w, float* dw, float scale, int accumulate, unsigned zero_blocks) {
   NRS_PDL_PROLOGUE();
+  // The blocks that write zeros are spread among those that sum.
+  const unsigned zeros_before = (unsigned)((uint64_t)blockIdx.x * zero_blocks / gridDim.x);
+  if ((unsigned)((uint64_t)(blockIdx.x + 1) * zero_blocks / gridDim.x) != zeros_before) {
+    const int r0 = (int)zeros_before * kZeroRows, r1 = min(p.vocab, r0 + kZeroRows);
+    for (int r = r0 + (threadIdx.x >> 5); r < r1; r += kSumWarps) {
+      if (w.start[r] != w.start[r + 1]) continue;
+      float* row = dw + (size_t)r * p.dim;
+      if (VEC)
+        for (int c = threadIdx.x & 31; c < p.dim / 4; c += 32) reinterpret_cast<float4*>(row)[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      else
+        for (int c = threadIdx.x & 31; c < p.dim; c += 32) row[c] = 0.0f;
+    }
+    return;
+  }
+  const unsigned block = blockIdx.x - zeros_before;
   __shared__ float4 s_head[kSumWarps][32], s_tail[kSumWarps][32];
+  __shared__ int s_last[2];                        // ids whose pieces' sums this block adds up
   __shared__ int s_flags[kSumWarps];               // 1: has a sum for a run from before; 2: for one that goes on; 4: both are one run
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int piece = blockIdx.x / p.slabs, slab = blockIdx.x - piece * p.slabs;
+  const int piece = block / p.slabs, slab = block - piece * p.slabs;
   const Cols<VEC> cols{slab * kSlab + (VEC ? 4 * lane : lane), p.dim};
-  const int valid = w.start[p.vocab];              // tokens with an id of the vocabulary
-  const int base = piece * p.piece() + warp * p.per_warp, n = min(p.per_warp, valid - base);
+  const int base = piece * p.piece() + warp * p.per_warp;
+  // (loaded together: the pairs behind the last valid one are not looked at)
+  const int edge_at = lane == 0 ? base - 1 : base + p.per_warp;
+  const int2 pair = base + lane < p.tokens && lane < p.per_warp ? w.sorted[base + lane] : make_int2(-1, 0);
+  const int beside = lane < 2 && edge_at >= 0 && edge_at < p.tokens ? w.sorted[edge_at].x : -1;
+  const int valid = w.start[p.vocab], n = min(p.per_warp, valid - base);   // valid: tokens with an id of the vocabulary
 
   auto finish = [&](int id, const float (&a)[4]) {   // a row's sum is complete
     float* row = dw + (size_t)id * p.dim;
@@ -278,8 +273,8 @@ embed_sum_kernel(const float* __restrict__ g, const Plan p, const Work w, float*
 
   int flags = 0, id_first = -1, id_last = -1;
   if (n > 0) {
-    const int2 e = lane < n ? w.sorted[base + lane] : make_int2(-1, 0);
-    const int edge = lane == 0 ? (base > 0 ? w.sorted[base - 1].x : -1) : lane == 1 ? (base + n < valid ? w.sorted[base + n].x : -1) : 0;
+    const int2 e = lane < n ? pair : make_int2(-1, 0);
+    const int edge = lane == 1 && base + n >= valid ? -1 : beside;
     id_first = __shfl_sync(0xffffffffu, e.x, 0);
     id_last = __shfl_sync(0xffffffffu, e.x, n - 1);
     const bool from_before = __shfl_sync(0xffffffffu, edge, 0) == id_first, goes_on = __shfl_sync(0xffffffffu, edge, 1) == id_last;
@@ -325,6 +320,7 @@ embed_sum_kernel(const float* __restrict__ g, const Plan p, const Work w, float*
     }
   }
   if (lane == 0) s_flags[warp] = flags;
+  if (threadIdx.x < 2) s_last[threadIdx.x] = -1;
   __syncthreads();
 
   // The sums of one run that lie in several warps: added up by the warp where it starts, or (a run from an earlier piece)
@@ -348,30 +344,49 @@ embed_sum_kernel(const float* __restrict__ g, const Plan p, const Work w, float*
     cols.store(a, w.partial + ((size_t)piece * 2 + (incoming ? 0 : 1)) * p.dim);
     __threadfence();
     __syncwarp();
-    unsigned done = 0;
-    if (lane == 0) done = atomicAdd(&w.tickets[(size_t)from * p.slabs + slab], 1u);
-    if (__shfl_sync(0xffffffffu, done, 0) != (unsigned)(to - from)) return;
-    __threadfence();
-    cols.load(a, w.partial + ((size_t)from * 2 + 1) * p.dim);
-    constexpr int kDeep = 8;
-    for (int k0 = from + 1; k0 <= to; k0 += kDeep) {
-      float v[kDeep][4];
-#pragma unroll
-      for (int k = 0; k < kDeep; ++k) {
-        if (k0 + k > to) break;
-        cols.load(v[k], w.partial + (size_t)(k0 + k) * 2 * p.dim);
-      }
-#pragma unroll
-      for (int k = 0; k < kDeep; ++k) {
-        if (k0 + k > to) break;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] += v[k][j];
-      }
+    if (lane == 0 && atomicAdd(&w.tickets[(size_t)from * p.slabs + slab], 1u) == (unsigned)(to - from)) {
+      s_last[incoming ? 0 : 1] = id;
+      __threadfence();
     }
-    finish(id, a);
   };
   if (warp == 0 && (flags & 1)) chain(true);
   if (flags & 2) chain(false);
+  __syncthreads();
+  // Such a sum: every warp adds a stretch of the pieces, the first the stretches.  (By one warp the 512 pieces of a token that
+  // is everywhere take 44 us.)
+  for (int which = 0; which < 2; ++which) {
+    const int id = s_last[which];
+    if (id < 0) continue;
+    const int from = w.start[id] / p.piece(), to = (w.start[id + 1] - 1) / p.piece(), each = (to - from + kSumWarps) / kSumWarps;
+    const int k0 = from + warp * each, k1 = min(to + 1, k0 + each);
+    float a[4] = {};
+    constexpr int kDeep = 8;
+    for (int k = k0; k < k1; k += kDeep) {
+      float v[kDeep][4];
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) {
+        if (k + i >= k1) break;
+        cols.load(v[i], w.partial + ((size_t)(k + i) * 2 + (k + i == from ? 1 : 0)) * p.dim);
+      }
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) {
+        if (k + i >= k1) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] += v[i][j];
+      }
+    }
+    s_head[warp][lane] = make_float4(a[0], a[1], a[2], a[3]);
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int k = 1; k < kSumWarps; ++k) {
+        const float4 o = s_head[k][lane];
+        a[0] += o.x; a[1] += o.y; a[2] += o.z; a[3] += o.w;
+      }
+      finish(id, a);
+    }
+    __syncthreads();
+  }
 }
 
 }  // namespace
@@ -415,17 +430,17 @@ int nrs_embedding_sorted_bwd(nrs_ctx* ctx, const float* g, const int32_t* idx, f
   const size_t need = work_of(p, workspace, &w);
   NRS_REQUIRE(ctx, workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, NRS_ERR_ARG,
               "%s: needs a workspace of %zu bytes on a 16-byte boundary", __func__, need);
-  NRS_REQUIRE(ctx, (long)p.pieces * p.slabs <= 0x7fffffffL, NRS_ERR_SHAPE, "%s: %d tokens of %d features are too many for one call", __func__, tokens, dim);
+  NRS_REQUIRE(ctx, (long)p.pieces * p.slabs + vocab <= 0x7fffffffL, NRS_ERR_SHAPE, "%s: %d tokens of %d features are too many for one call", __func__, tokens, dim);
   NrsDeviceGuard on(ctx);
   const bool vec = dim % 4 == 0 && (((uintptr_t)g | (uintptr_t)dweight) & 15) == 0;
-  const size_t smem = sizeof(int2) * kTile + sizeof(int) * p.range;
+  const size_t smem = sizeof(int) * kSortWarps * p.range;
   static NrsSmemAttr attr;
   NRS_ENSURE_SMEM(ctx, attr, embed_sort_kernel, smem);
-  NRS_PDL_LAUNCH(embed_sort_kernel, (vocab + p.range - 1) / p.range, kSortThreads, smem, ctx->stream, idx, p, w, accumulate ? nullptr : dweight, vec);
+  NRS_PDL_LAUNCH(embed_sort_kernel, (vocab + p.range - 1) / p.range, kSortThreads, smem, ctx->stream, idx, p, w);
   NRS_LAUNCHED(ctx);
-  if (tokens == 0) return NRS_OK;
-  if (vec) NRS_PDL_LAUNCH(embed_sum_kernel<true>, p.pieces * p.slabs, kSumWarps * 32, 0, ctx->stream, g, p, w, dweight, scale, accumulate != 0);
-  else NRS_PDL_LAUNCH(embed_sum_kernel<false>, p.pieces * p.slabs, kSumWarps * 32, 0, ctx->stream, g, p, w, dweight, scale, accumulate != 0);
+  const unsigned zeros = accumulate ? 0 : (unsigned)((vocab + kZeroRows - 1) / kZeroRows), blocks = (unsigned)(p.pieces * p.slabs) + zeros;
+  if (vec) NRS_PDL_LAUNCH(embed_sum_kernel<true>, blocks, kSumWarps * 32, 0, ctx->stream, g, p, w, dweight, scale, accumulate != 0, zeros);
+  else NRS_PDL_LAUNCH(embed_sum_kernel<false>, blocks, kSumWarps * 32, 0, ctx->stream, g, p, w, dweight, scale, accumulate != 0, zeros);
   NRS_LAUNCHED(ctx);
   return NRS_OK;
 }
