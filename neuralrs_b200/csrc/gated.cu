@@ -2,7 +2,8 @@
 // form of the FP32 and TF32 modes and of layers too small for the tensor cores.  No reference counterpart (its feed-forward
 // is ungated, src/cuda/nn/transformer_block.rs:37-40).
 //
-// Up to 15 rows (tokens that are being generated): bound by the weights, 8 k n bytes read once.  A block owns 32 columns of
+// Up to 15 rows (tokens that are being generated; 5 and more of a large layer take gated_skinny.cu): bound by the weights, 8 k n
+// bytes read once.  A block owns 32 columns of
 // both matrices and a share of k; its warps read four rows of 128 bytes with each load of either matrix, four loads of each
 // under way, against values of x in shared memory.  The shares of k are the CTAs of a cluster, which add their sums up
 // through distributed shared memory: with 2752 columns there are 86 blocks of columns for 148 SMs.
@@ -145,6 +146,19 @@ int few_rows(nrs_ctx* ctx, const Shape& s, const float* x, const float* wg, cons
   return NRS_OK;
 }
 
+// Where the tensor-core form without a pass over the weights is the fastest (us; few rows, that one, staged operands):
+//   rows  k x n         few   this  staged        rows  k x n        this  staged
+//   4     2048 x 5504   25.0  24.1                 16   2048 x 5504   26.2  78.4
+//   8     2048 x 5504   55.2  25.8                128   2048 x 5504   56.5  80.1
+//   8     1024 x 2752   15.9  11.0                200   2048 x 5504   98.6  92.6
+//   8     2048 x 700    10.0  10.0                128   256 x 1024    10.8  12.7
+//   8     512 x 1000     7.2   7.1                 32   100 x 5000    10.8  11.8
+//   8     100 x 5000     6.2   9.8                 64   100 x 5000    13.6  12.1
+bool skinny(const Shape& s) {
+  if (s.m <= kFewRows) return s.m > 4 && (double)s.m * s.n * s.k >= 8e6;
+  return s.m <= 32 || (s.m <= 128 && s.k >= 256);
+}
+
 // h = act(a) u, element by element.
 __global__ void __launch_bounds__(256) gated_act_kernel(const float* __restrict__ a, const float* __restrict__ u, float* __restrict__ h, size_t total, int act) {
   NRS_PDL_PROLOGUE();
@@ -200,6 +214,10 @@ int nrs_gated_linear_fwd(nrs_ctx* ctx, const float* x, const float* w_gate, cons
     return NRS_OK;
   }
   const Shape s{m, n, k, act};
+  if (skinny(s)) {
+    st = nrs_gated_skinny_fwd(ctx, s, x, w_gate, w_up, h, pre_gate, pre_up);
+    if (st != NRS_ERR_UNSUPPORTED) return st;
+  }
   if (m <= kFewRows) return few_rows(ctx, s, x, w_gate, w_up, h, pre_gate, pre_up);
   st = nrs_tc_gated_fwd(ctx, s, x, w_gate, w_up, h, pre_gate, pre_up);
   if (st != NRS_ERR_UNSUPPORTED) return st;

@@ -48,3 +48,5 @@ struct Shape { int m, n, k, act; };
 int nrs_tc_gated_fwd(nrs_ctx* ctx, const gated::Shape& s, const float* x, const float* w_gate, const float* w_up, float* h, float* pre_gate, float* pre_up);
 int nrs_tc_gated_bwd(nrs_ctx* ctx, const gated::Shape& s, const float* x, const float* w_gate, const float* w_up, const float* pre_gate, const float* pre_up,
                      const float* dh, float* dx, float* dw_gate, float* dw_up, int acc_x, int acc_w);
+// The forward pass of some dozen rows (gated_skinny.cu); NRS_ERR_UNSUPPORTED (no error text) likewise.
+int nrs_gated_skinny_fwd(nrs_ctx* ctx, const gated::Shape& s, const float* x, const float* w_gate, const float* w_up, float* h, float* pre_gate, float* pre_up);

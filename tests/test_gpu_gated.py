@@ -80,7 +80,8 @@ def unit(mode, k):
 
 
 SHAPES = [(1, 1, 1), (1, 128, 64), (1, 2752, 1024), (2, 33, 65), (3, 100, 37), (5, 96, 2000), (15, 64, 300), (15, 70, 31), (16, 31, 40), (16, 64, 64), (17, 33, 35),
-          (64, 32, 32), (100, 200, 72), (129, 129, 129), (128, 64, 1024), (300, 500, 777), (1000, 96, 64), (257, 1024, 320), (40, 2000, 2000), (2500, 72, 40)]
+          (64, 32, 32), (100, 200, 72), (129, 129, 129), (128, 64, 1024), (300, 500, 777), (1000, 96, 64), (257, 1024, 320), (40, 2000, 2000), (2500, 72, 40),
+          (5, 2000, 1000), (9, 1000, 1000), (15, 68, 8000), (32, 100, 100), (33, 260, 300), (128, 1000, 260), (127, 68, 500), (100, 64, 2500)]
 
 
 @pytest.mark.gpu
