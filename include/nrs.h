@@ -398,7 +398,7 @@ int nrs_embedding_bwd(nrs_ctx* ctx, const float* g, const int32_t* idx, float* d
  * scale * the sum of g[t,:] over the tokens with idx[t] == v, in one fixed order (deterministic).  An id outside the
  * vocabulary contributes nothing.  accumulate == 0 writes every row of dweight, zeros where no token is.  The workspace, at
  * least nrs_embedding_sorted_workspace bytes, is used by this call alone: calls that may run at the same time (two
- * captured graphs) bring one each.  tokens up to 2^30. */
+ * captured graphs) bring one each.  tokens and vocab up to 2^30. */
 int nrs_embedding_scaled_fwd(nrs_ctx* ctx, const float* weight, const int32_t* idx, const float* pos_table, float* out,
                              int tokens, int seq, int dim, int vocab, float scale);
 size_t nrs_embedding_sorted_workspace(int tokens, int dim, int vocab);

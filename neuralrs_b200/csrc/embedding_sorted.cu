@@ -21,6 +21,7 @@
 // Deterministic: every sum has one order, whatever the blocks' timing.  Bound by memory: g read once, dweight written once.
 #include <algorithm>
 
+#include "igemm_problems.cuh"
 #include "nrs_internal.h"
 
 namespace {
@@ -29,32 +30,44 @@ constexpr int kErrBadIndex = 5;
 
 // ------------------------------------------------------------------------------------------------ lookup
 
-// One vector (VEC: 16 bytes) of a row per thread and step, four under way together.
-template <bool VEC>
+// One vector (VEC: 16 bytes) of a row per thread and step, four under way together.  WIDE: more of them than fast division
+// takes.
+template <bool VEC, bool WIDE>
 __global__ void __launch_bounds__(256)
 embed_scaled_kernel(const float* __restrict__ w, const int32_t* __restrict__ idx, const float* __restrict__ pos, float* __restrict__ out, size_t total,
-                    int width /*vectors of a row*/, int seq, int vocab, float scale, int* err) {
+                    int width /*vectors of a row*/, NrsFastDiv by_width, NrsFastDiv by_seq, int vocab, float scale, int* err) {
   NRS_PDL_PROLOGUE();
   constexpr int kDeep = 4;
   const size_t stride = (size_t)gridDim.x * blockDim.x;
   for (size_t i0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i0 < total; i0 += kDeep * stride) {
     float4 v[kDeep], p[kDeep];
+    uint32_t t[kDeep], c[kDeep];
+    int row[kDeep];
 #pragma unroll
     for (int k = 0; k < kDeep; ++k) {
-      const size_t i = i0 + k * stride;
+      const size_t i = min(i0 + k * stride, total - 1);   // (past the end: the last one again)
+      if (WIDE) {
+        t[k] = (uint32_t)(i / (size_t)width);
+        c[k] = (uint32_t)(i - (size_t)t[k] * width);
+      } else {
+        by_width.divmod((uint32_t)i, t[k], c[k]);
+      }
+      row[k] = idx[t[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
       v[k] = p[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (i >= total) continue;
-      const size_t t = (i >> 32) ? i / (size_t)width : (size_t)((uint32_t)i / (uint32_t)width);
-      const int c = (int)(i - t * width), row = idx[t];
-      if (row >= 0 && row < vocab) {
-        const size_t at = (size_t)row * width + c;
+      if (row[k] >= 0 && row[k] < vocab) {
+        const size_t at = (size_t)row[k] * width + c[k];
         if (VEC) v[k] = reinterpret_cast<const float4*>(w)[at];
         else v[k].x = w[at];
-      } else if (c == 0) {
+      } else if (c[k] == 0) {
         atomicExch(err, kErrBadIndex);
       }
       if (pos) {
-        const size_t at = (size_t)((uint32_t)t % (uint32_t)seq) * width + c;
+        uint32_t q, r;
+        by_seq.divmod(t[k], q, r);
+        const size_t at = (size_t)r * width + c[k];
         if (VEC) p[k] = reinterpret_cast<const float4*>(pos)[at];
         else p[k].x = pos[at];
       }
@@ -62,7 +75,7 @@ embed_scaled_kernel(const float* __restrict__ w, const int32_t* __restrict__ idx
 #pragma unroll
     for (int k = 0; k < kDeep; ++k) {
       const size_t i = i0 + k * stride;
-      if (i >= total) continue;
+      if (i >= total) break;
       if (VEC) reinterpret_cast<float4*>(out)[i] = make_float4(fmaf(scale, v[k].x, p[k].x), fmaf(scale, v[k].y, p[k].y), fmaf(scale, v[k].z, p[k].z),
                                                                fmaf(scale, v[k].w, p[k].w));
       else out[i] = fmaf(scale, v[k].x, p[k].x);
@@ -212,6 +225,16 @@ struct Cols {
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = c0 + 32 * j < dim ? row[c0 + 32 * j] : 0.0f;
+    }
+  }
+  // The same of what another block has written.
+  __device__ __forceinline__ void load_shared(float (&v)[4], const float* row) const {
+    if (VEC) {
+      const float4 q = c0 < dim ? __ldcg(reinterpret_cast<const float4*>(row + c0)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = c0 + 32 * j < dim ? __ldcg(row + c0 + 32 * j) : 0.0f;
     }
   }
   __device__ __forceinline__ void store(const float (&v)[4], float* row) const {
@@ -366,7 +389,7 @@ embed_sum_kernel(const float* __restrict__ g, const Plan p, const Work w, float*
 #pragma unroll
       for (int i = 0; i < kDeep; ++i) {
         if (k + i >= k1) break;
-        cols.load(v[i], w.partial + ((size_t)(k + i) * 2 + (k + i == from ? 1 : 0)) * p.dim);
+        cols.load_shared(v[i], w.partial + ((size_t)(k + i) * 2 + (k + i == from ? 1 : 0)) * p.dim);
       }
 #pragma unroll
       for (int i = 0; i < kDeep; ++i) {
@@ -408,8 +431,15 @@ int nrs_embedding_scaled_fwd(nrs_ctx* ctx, const float* weight, const int32_t* i
   const int width = vec ? dim / 4 : dim;
   const size_t total = (size_t)tokens * width, want = (total + 255) / 256, cap = (size_t)ctx->sm_count * 16;
   const unsigned blocks = (unsigned)(want < cap ? want : cap);
-  if (vec) NRS_PDL_LAUNCH(embed_scaled_kernel<true>, blocks, 256, 0, ctx->stream, weight, idx, pos_table, out, total, width, seq > 0 ? seq : 1, vocab, scale, err);
-  else NRS_PDL_LAUNCH(embed_scaled_kernel<false>, blocks, 256, 0, ctx->stream, weight, idx, pos_table, out, total, width, seq > 0 ? seq : 1, vocab, scale, err);
+  const bool wide = total > 0x7fffffffu;
+  const NrsFastDiv by_width(width), by_seq(pos_table ? seq : 1);
+#define NRS_EMBED(VEC_, WIDE_) \
+  NRS_PDL_LAUNCH((embed_scaled_kernel<VEC_, WIDE_>), blocks, 256, 0, ctx->stream, weight, idx, pos_table, out, total, width, by_width, by_seq, vocab, scale, err)
+  if (vec && !wide) NRS_EMBED(true, false);
+  else if (vec) NRS_EMBED(true, true);
+  else if (!wide) NRS_EMBED(false, false);
+  else NRS_EMBED(false, true);
+#undef NRS_EMBED
   NRS_LAUNCHED(ctx);
   return NRS_OK;
 }
@@ -422,7 +452,7 @@ size_t nrs_embedding_sorted_workspace(int tokens, int dim, int vocab) {
 int nrs_embedding_sorted_bwd(nrs_ctx* ctx, const float* g, const int32_t* idx, float* dweight, int tokens, int dim, int vocab, float scale, int accumulate,
                              void* workspace, size_t workspace_bytes) {
   NRS_REQUIRE_CTX(ctx);
-  NRS_REQUIRE(ctx, tokens >= 0 && dim > 0 && vocab > 0 && tokens <= (1 << 30), NRS_ERR_SHAPE, "%s: bad shape [%d,%d], vocabulary %d", __func__, tokens, dim, vocab);
+  NRS_REQUIRE(ctx, tokens >= 0 && dim > 0 && vocab > 0 && tokens <= (1 << 30) && vocab <= (1 << 30), NRS_ERR_SHAPE, "%s: bad shape [%d,%d], vocabulary %d", __func__, tokens, dim, vocab);
   if (tokens == 0 && accumulate) return NRS_OK;
   NRS_REQUIRE(ctx, dweight && (tokens == 0 || (g && idx)), NRS_ERR_ARG, "%s: null tensor", __func__);
   const Plan p = plan_of(tokens, dim, vocab, ctx->sm_count);

@@ -5,15 +5,17 @@
 
 namespace gated {
 
-// 1 / (1 + exp(-v)), and exp(-v) itself, kept finite.  The exponential as a power of two, 2 ulp, of -v log2(e) taken in two
-// parts (its rounding error is put back to first order), and the quotient within 2 ulp: a third of the instructions that
-// expf and a correctly rounded division take, which is what these element-wise passes were bound by.
+// 1 / (1 + exp(-v)), and exp(-v) itself, kept finite.  The exponential as the hardware's power of two, 2 ulp, of -v log2(e)
+// taken in two parts (its rounding error is put back to first order), and its reciprocal, 1 ulp: a third of the instructions
+// that expf and a correctly rounded division take, which is what these element-wise passes were bound by.
 __device__ __forceinline__ float sigmoid(float v, float& e) {
   constexpr float kLog2e = 1.4426950408889634f, kRest = (float)(1.4426950408889634 - (double)kLog2e), kLn2 = 0.6931471805599453f;
   const float x = fmaxf(fminf(-v, 80.0f), -120.0f), t = x * kLog2e, rest = fmaf(x, kRest, fmaf(x, kLog2e, -t));
-  const float p = exp2f(t);
+  float p, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
   e = fmaf(p, rest * kLn2, p);
-  return __fdividef(1.0f, 1.0f + e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + e));
+  return s;
 }
 // act(a) and its derivative.  SiLU is a s with s = sigmoid(a), GELU (the tanh form) with s = sigmoid(2 u), u = sqrt(2/pi) (a +
 // 0.044715 a^3); with w the sigmoid's argument the derivative is s + a s (1 - s) dw/da, and 1 - s = e s cancels nowhere.

@@ -269,8 +269,10 @@ int run(nrs_ctx* ctx, const Shape& s, const float* x, const float* wg, const flo
   // At least two slices a CTA.
   const long ctas = std::min<long>(ctx->sm_count, std::max<long>(1, wk.total / 2)), least = wk.total / ctas;
   wk.slots_max = (int)((wk.per_tile + least - 1) / least + 1);
+  const size_t scratch = sizeof(float) * tiles * wk.slots_max * N * 128;
+  if (scratch > ((size_t)256 << 20)) return NRS_ERR_UNSUPPORTED;   // (hundreds of thousands of columns)
   void* p = nullptr;
-  int st = nrs_ws_slot(ctx, NRS_WS_PARTIAL, sizeof(float) * tiles * wk.slots_max * N * 128, &p);
+  int st = nrs_ws_slot(ctx, NRS_WS_PARTIAL, scratch, &p);
   if (st != NRS_OK) return st;
   wk.partial = (float*)p;
   int* err = nullptr;

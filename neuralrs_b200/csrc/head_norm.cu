@@ -373,6 +373,8 @@ struct Shape { int tokens, seq, heads_q, heads_k, d, rot, max_len, interleaved; 
 int check_shape(nrs_ctx* ctx, const char* who, const Shape& s, const float* table, const int32_t* positions) {
   NRS_REQUIRE(ctx, s.tokens >= 0 && s.heads_q >= 0 && s.heads_k >= 0 && s.d > 0, NRS_ERR_SHAPE, "%s: bad shape: %d tokens, %d and %d heads of %d", who,
               s.tokens, s.heads_q, s.heads_k, s.d);
+  NRS_REQUIRE(ctx, (long)s.heads_q * s.d <= 0x7fffffffL && (long)s.heads_k * s.d <= 0x7fffffffL, NRS_ERR_SHAPE, "%s: a row of %d or %d heads of %d", who, s.heads_q,
+              s.heads_k, s.d);
   NRS_REQUIRE(ctx, s.d <= kMaxHead, NRS_ERR_UNSUPPORTED, "%s: heads of %d features (at most %d)", who, s.d, kMaxHead);
   NRS_REQUIRE(ctx, s.eps >= 0.0f, NRS_ERR_ARG, "%s: negative eps", who);
   if (!table) {

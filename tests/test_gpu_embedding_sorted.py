@@ -200,7 +200,7 @@ def test_refusals(gpu_ctx):
     need = _lib.lib().nrs_embedding_sorted_workspace(8, 4, 10)
     ok = dict(g=b, idx=ids, dw=b, t=8, d=4, v=10, ws=b, n=need)
     for change, code in [(dict(g=None), 1), (dict(idx=None), 1), (dict(dw=None), 1), (dict(ws=None), 1), (dict(n=need - 1), 1), (dict(t=-1), 2), (dict(d=0), 2),
-                         (dict(v=0), 2), (dict(ws=C.c_void_p(b.ptr.value + 4)), 1), (dict(t=(1 << 30) + 1), 2)]:
+                         (dict(v=0), 2), (dict(ws=C.c_void_p(b.ptr.value + 4)), 1), (dict(t=(1 << 30) + 1), 2), (dict(v=(1 << 30) + 1), 2)]:
         a = {**ok, **change}
         with pytest.raises(_lib.NrsError) as e:
             call(gpu_ctx, "nrs_embedding_sorted_bwd", a["g"], a["idx"], a["dw"], a["t"], a["d"], a["v"], F(1.0), 0, a["ws"], a["n"])

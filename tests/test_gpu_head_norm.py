@@ -334,7 +334,7 @@ def test_refusals(gpu_ctx):
                      (dict(shape=(4, 9, 2, 0, 32, 31, 8, 0, F(EPS))), 2), (dict(shape=(4, 4, 2, 0, 32, 34, 8, 0, F(EPS))), 2),
                      (dict(shape=(9, 9, 2, 0, 32, 32, 8, 0, F(EPS))), 2), (dict(shape=(4, 0, 2, 0, 32, 32, 8, 0, F(EPS))), 2),
                      (dict(shape=(-1, 4, 2, 0, 32, 32, 8, 0, F(EPS))), 2), (dict(shape=(4, 4, 2, 0, 1025, 32, 8, 0, F(EPS))), 7),
-                     (dict(shape=(4, 4, 2, 0, 32, 32, 8, 0, F(-1.0))), 1)]:
+                     (dict(shape=(4, 4, 2, 0, 32, 32, 8, 0, F(-1.0))), 1), (dict(shape=(1, 1, 1 << 27, 0, 32, 32, 8, 0, F(EPS))), 2)]:
         with pytest.raises(_lib.NrsError) as e:
             fwd(**kw)
         assert e.value.code == code, kw
