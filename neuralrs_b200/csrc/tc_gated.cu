@@ -149,8 +149,8 @@ struct Job {
   int rows, cols, pad;      // pad: a row's values in the planes, cols rounded up to 64
   long ld;                  // values between rows of the planes
   unsigned first, blocks;   // of the launch
-  NrsFastDiv div;           // of pad / 8
-  bool vec;
+  NrsFastDiv div;           // of a row's units
+  bool vec, whole;          // rows, or the tensor at least, start on 16 bytes
 };
 struct Jobs {
   Job j[4];
@@ -174,75 +174,127 @@ __device__ __forceinline__ void put8(__half* hi, __half* lo, size_t at, const fl
   *reinterpret_cast<uint4*>(lo + at) = make_uint4(l0.x, l0.y, l1.x, l1.y);
 }
 
-// MEASURE: the largest magnitude of each tensor into its range.  Of da and du: of dh u, times 1.13, which no activation's
-// slope exceeds, and of dh a, which no activation exceeds; without their exponentials this is a pass at memory speed.
-// Otherwise the pairs, zeros from cols to pad.
-template <bool MEASURE>
-__global__ void __launch_bounds__(256, MEASURE ? 3 : 4) gated_stage_kernel(const Jobs jobs) {
-  NRS_PDL_PROLOGUE();
+__device__ __forceinline__ const Job& job_of(const Jobs& jobs) {
   int which = 0;
   while (which + 1 < jobs.count && blockIdx.x >= jobs.j[which + 1].first) ++which;
-  const Job& q = jobs.j[which];
-  const uint32_t units = (uint32_t)q.rows * (uint32_t)(q.pad / 8), step = q.blocks * 256;   // (the launcher checks the range)
+  return jobs.j[which];
+}
+
+// The largest magnitude of each tensor into its range.  Of da and du: of dh u, times 1.13, which no activation's slope exceeds,
+// and of dh a, which no activation exceeds; without their exponentials this is a pass at memory speed.
+__global__ void __launch_bounds__(256, 3) gated_measure_kernel(const Jobs jobs) {
+  NRS_PDL_PROLOGUE();
+  const Job& q = job_of(jobs);
+  const size_t count = (size_t)q.rows * q.cols, units = q.whole ? count / 8 : 0, step = (size_t)q.blocks * 256;   // (whole: 16-byte accesses)
   const bool grads = q.a != nullptr;
-  const float bound = MEASURE ? 0.0f : q.range->top, scale = MEASURE ? 1.0f : pr::scale_of(bound);
-  if (!MEASURE && blockIdx.x == q.first && threadIdx.x == 0) q.range->bound = bound;
   uint32_t top = 0;
-  constexpr int kDeep = MEASURE ? 2 : 1;
-  for (uint32_t i0 = (blockIdx.x - q.first) * 256 + threadIdx.x; i0 < units; i0 += kDeep * step) {
+  auto see = [&](float (&g)[8], float (&a)[8], float (&u)[8]) {
+    if (grads) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        u[i] *= 1.13f * g[i];
+        a[i] *= g[i];
+      }
+      top = pr::seen_all(top, u);
+      top = pr::seen_all(top, a);
+    } else {
+      top = pr::seen_all(top, g);
+    }
+  };
+  const size_t me = (size_t)(blockIdx.x - q.first) * 256 + threadIdx.x;
+  constexpr int kDeep = 2;
+  for (size_t i0 = me; i0 < units; i0 += kDeep * step) {
     float g[kDeep][8], a[kDeep][8], u[kDeep][8];
-    uint32_t row[kDeep], col[kDeep];
 #pragma unroll
     for (int k = 0; k < kDeep; ++k) {
-      const uint32_t i = min(i0 + k * step, units - 1);   // (past the end: the last one again)
-      q.div.divmod(i, row[k], col[k]);
-      col[k] *= 8;
-      const int left = q.cols - (int)col[k];
-      const size_t at = (size_t)row[k] * q.cols + col[k];
-      eight(g[k], q.src + at, left, q.vec);
+      const size_t at = 8 * min(i0 + k * step, units - 1);   // (past the end: the last one again)
+      eight(g[k], q.src + at, 8, true);
       if (grads) {
-        eight(a[k], q.a + at, left, q.vec);
-        eight(u[k], q.u + at, left, q.vec);
+        eight(a[k], q.a + at, 8, true);
+        eight(u[k], q.u + at, 8, true);
       }
     }
 #pragma unroll
-    for (int k = 0; k < kDeep; ++k) {
-      if (k > 0 && i0 + k * step >= units) break;
-      const size_t at = (size_t)row[k] * q.ld + col[k];
-      if (MEASURE) {
-        if (grads) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            u[k][i] *= 1.13f * g[k][i];
-            a[k][i] *= g[k][i];
-          }
-          top = pr::seen_all(top, u[k]);
-          top = pr::seen_all(top, a[k]);
-        } else {
-          top = pr::seen_all(top, g[k]);
-        }
-      } else if (grads) {
-        float da[8], du[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float f, d;
-          gated::act_both(a[k][i], jobs.act, f, d);
-          da[i] = g[k][i] * u[k][i] * d;
-          du[i] = g[k][i] * f;
-        }
-        put8(q.hi, q.lo, at, da, scale);
-        put8(q.hi, q.lo, at + q.pad, du, scale);
-      } else {
-        put8(q.hi, q.lo, at, g[k], scale);
-      }
-    }
+    for (int k = 0; k < kDeep; ++k) see(g[k], a[k], u[k]);
   }
-  if (MEASURE) {   // (one atomic a block: those of ten thousand warps on one word took longer than the pass)
-    __shared__ uint32_t tops[8];
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-    __syncthreads();
-    if (threadIdx.x < 32) pr::report(q.range, threadIdx.x < 8 ? tops[threadIdx.x] : 0u);
+  for (size_t i = 8 * units + me; i < count; i += step) {   // what is left of them, or all
+    float g[8] = {q.src[i]}, a[8] = {}, u[8] = {};
+    if (grads) { a[0] = q.a[i]; u[0] = q.u[i]; }
+    see(g, a, u);
+  }
+  // (one atomic a block: those of ten thousand warps on one word took longer than the pass)
+  __shared__ uint32_t tops[8];
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x < 32) pr::report(q.range, threadIdx.x < 8 ? tops[threadIdx.x] : 0u);
+}
+
+// The pairs, zeros from cols to pad: eight values a thread where rows start on 16 bytes, else 128 values a warp, value by value
+// (eight neighbours a thread, loaded one by one, touch eight lines with every load).
+__global__ void __launch_bounds__(256, 4) gated_stage_kernel(const Jobs jobs) {
+  NRS_PDL_PROLOGUE();
+  const Job& q = job_of(jobs);
+  const bool grads = q.a != nullptr;
+  const float bound = q.range->top, scale = pr::scale_of(bound);
+  if (blockIdx.x == q.first && threadIdx.x == 0) q.range->bound = bound;
+  if (q.vec) {
+    const uint32_t units = (uint32_t)q.rows * (uint32_t)(q.pad / 8), step = q.blocks * 256;   // (the launcher checks the range)
+    for (uint32_t i = (blockIdx.x - q.first) * 256 + threadIdx.x; i < units; i += step) {
+      uint32_t row, col;
+      q.div.divmod(i, row, col);
+      col *= 8;
+      const int left = q.cols - (int)col;
+      const size_t from = (size_t)row * q.cols + col, at = (size_t)row * q.ld + col;
+      float g[8];
+      eight(g, q.src + from, left, true);
+      if (!grads) {
+        put8(q.hi, q.lo, at, g, scale);
+        continue;
+      }
+      float a[8], u[8];
+      eight(a, q.a + from, left, true);
+      eight(u, q.u + from, left, true);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float f, d;
+        gated::act_both(a[k], jobs.act, f, d);
+        a[k] = g[k] * u[k] * d;
+        u[k] = g[k] * f;
+      }
+      put8(q.hi, q.lo, at, a, scale);
+      put8(q.hi, q.lo, at + q.pad, u, scale);
+    }
+    return;
+  }
+  const uint32_t units = (uint32_t)q.rows * (uint32_t)((q.pad + 127) / 128), step = q.blocks * 8;
+  for (uint32_t i = (blockIdx.x - q.first) * 8 + (threadIdx.x >> 5); i < units; i += step) {
+    uint32_t row, seg;
+    q.div.divmod(i, row, seg);
+    const int c0 = (int)seg * 128 + (threadIdx.x & 31);
+    const size_t from = (size_t)row * q.cols + c0, at = (size_t)row * q.ld + c0;
+    float g[4], a[4] = {}, u[4] = {};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool on = c0 + 32 * k < q.cols;
+      g[k] = on ? q.src[from + 32 * k] : 0.0f;
+      if (grads) {
+        a[k] = on ? q.a[from + 32 * k] : 0.0f;
+        u[k] = on ? q.u[from + 32 * k] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (c0 + 32 * k >= q.pad) break;
+      if (!grads) {
+        pr::put(q.hi, q.lo, at + 32 * k, g[k], scale);
+        continue;
+      }
+      float f, d;
+      gated::act_both(a[k], jobs.act, f, d);
+      pr::put(q.hi, q.lo, at + 32 * k, g[k] * u[k] * d, scale);
+      pr::put(q.hi, q.lo, at + q.pad + 32 * k, g[k] * f, scale);
+    }
   }
 }
 
@@ -270,24 +322,27 @@ void add_job(Jobs* jobs, const float* src, const float* a, const float* u, int r
   q.hi = (__half*)to.hi + (size_t)mat * to.pad; q.lo = (__half*)to.lo + (size_t)mat * to.pad;
   q.range = to.range;
   q.rows = rows; q.cols = cols; q.pad = to.pad; q.ld = to.ld;
-  q.div = NrsFastDiv(to.pad / 8);
-  q.vec = cols % 4 == 0 && aligned({src, a, u});
+  q.whole = aligned({src, a, u});
+  q.vec = q.whole && cols % 4 == 0;
+  q.div = NrsFastDiv(q.vec ? to.pad / 8 : (to.pad + 127) / 128);
 }
 // Blocks by the jobs' bytes, up to eight an SM in all (a job's own units permitting).
-template <bool MEASURE>
 int run_jobs(nrs_ctx* ctx, Jobs& jobs) {
-  double work[4], all = 0.0;
-  for (int i = 0; i < jobs.count; ++i) all += work[i] = (double)jobs.j[i].rows * jobs.j[i].pad * (jobs.j[i].a ? (MEASURE ? 3.0 : 5.0) : (MEASURE ? 1.0 : 2.0));
-  unsigned at = 0;
-  for (int i = 0; i < jobs.count; ++i) {
-    Job& q = jobs.j[i];
-    const unsigned most = (unsigned)(((size_t)q.rows * (q.pad / 8) + 255) / 256), share = (unsigned)(work[i] / all * 8 * ctx->sm_count) + 1;
-    q.first = at;
-    q.blocks = std::min(most, share);
-    at += q.blocks;
+  for (int pass = 0; pass < 2; ++pass) {   // measure, then write
+    double work[4], all = 0.0;
+    for (int i = 0; i < jobs.count; ++i) all += work[i] = (double)jobs.j[i].rows * jobs.j[i].pad * (jobs.j[i].a ? (pass ? 5.0 : 3.0) : (pass ? 2.0 : 1.0));
+    unsigned at = 0;
+    for (int i = 0; i < jobs.count; ++i) {
+      Job& q = jobs.j[i];
+      const unsigned most = (unsigned)(((size_t)q.rows * (q.pad / 8) + 255) / 256), share = (unsigned)(work[i] / all * 8 * ctx->sm_count) + 1;
+      q.first = at;
+      q.blocks = std::min(most, share);
+      at += q.blocks;
+    }
+    if (pass) NRS_PDL_LAUNCH(gated_stage_kernel, at, 256, 0, ctx->stream, jobs);
+    else NRS_PDL_LAUNCH(gated_measure_kernel, at, 256, 0, ctx->stream, jobs);
+    NRS_LAUNCHED(ctx);
   }
-  NRS_PDL_LAUNCH(gated_stage_kernel<MEASURE>, at, 256, 0, ctx->stream, jobs);
-  NRS_LAUNCHED(ctx);
   return NRS_OK;
 }
 
@@ -340,8 +395,7 @@ int nrs_tc_gated_fwd(nrs_ctx* ctx, const Shape& s, const float* x, const float* 
   add_job(&jobs, x, nullptr, nullptr, s.m, s.k, X, 0);
   add_job(&jobs, w_gate, nullptr, nullptr, s.k, s.n, W, 0);
   add_job(&jobs, w_up, nullptr, nullptr, s.k, s.n, W, 1);
-  st = run_jobs<true>(ctx, jobs);
-  if (st == NRS_OK) st = run_jobs<false>(ctx, jobs);
+  st = run_jobs(ctx, jobs);
   if (st != NRS_OK) return st;
   GatedPolicy<kForward> pol{};
   pol.out[0] = h; pol.pre[0] = pre_gate; pol.pre[1] = pre_up;
@@ -370,8 +424,7 @@ int nrs_tc_gated_bwd(nrs_ctx* ctx, const Shape& s, const float* x, const float* 
     add_job(&jobs, w_gate, nullptr, nullptr, s.k, s.n, W, 0);
     add_job(&jobs, w_up, nullptr, nullptr, s.k, s.n, W, 1);
   }
-  st = run_jobs<true>(ctx, jobs);
-  if (st == NRS_OK) st = run_jobs<false>(ctx, jobs);
+  st = run_jobs(ctx, jobs);
   if (st != NRS_OK) return st;
   int splits = 0;   // of the product for dx (0: there is none)
   if (dx) {
