@@ -148,11 +148,11 @@ int few_rows(nrs_ctx* ctx, const Shape& s, const float* x, const float* wg, cons
 
 // Where the tensor-core form without a pass over the weights is the fastest (us; few rows, that one, staged operands):
 //   rows  k x n         few   this  staged        rows  k x n        this  staged
-//   4     2048 x 5504   25.0  24.1                 16   2048 x 5504   26.2  78.4
-//   8     2048 x 5504   55.2  25.8                128   2048 x 5504   56.5  80.1
-//   8     1024 x 2752   15.9  11.0                200   2048 x 5504   98.6  92.6
-//   8     2048 x 700    10.0  10.0                128   256 x 1024    10.8  12.7
-//   8     512 x 1000     7.2   7.1                 32   100 x 5000    10.8  11.8
+//   4     2048 x 5504   25.0  24.1                 16   2048 x 5504   24.9  78.4
+//   8     2048 x 5504   55.2  24.7                128   2048 x 5504   52.8  80.1
+//   8     1024 x 2752   15.9  11.3                200   2048 x 5504   98.6  92.6
+//   8     2048 x 700    10.0   9.9                128   256 x 1024     9.3  12.7
+//   8     512 x 1000     7.2   7.2                 32   100 x 5000    10.8  11.8
 //   8     100 x 5000     6.2   9.8                 64   100 x 5000    13.6  12.1
 bool skinny(const Shape& s) {
   if (s.m <= kFewRows) return s.m > 4 && (double)s.m * s.n * s.k >= 8e6;

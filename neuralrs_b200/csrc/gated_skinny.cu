@@ -14,7 +14,7 @@
 // up in order, applies the activation and multiplies.
 //
 // A slice costs shared memory 16 KB in, 16 KB out and in again for the split, and 32 KB for the UMMAs' reads, about 730 clocks;
-// memory brings a slice in 710 when all SMs ask.  2048 -> 5504, 90 MB of weights (floor 14 us): 16 rows 26 us, 64 rows 36 us;
+// memory brings a slice in 710 when all SMs ask.  2048 -> 5504, 90 MB of weights (floor 14 us): 16 rows 25 us, 64 rows 34 us;
 // with one group of splitting warps, which then also drained, 31 and 41 us; measuring and staging the weights first 78 us.
 #include <algorithm>
 
@@ -99,9 +99,10 @@ gated_skinny_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_const
     // ---------------- TMA producer
     uint32_t s = 0, ph = 0, issued = 0;
     bool ok = true;
+    const int tile0 = (int)(begin / wk.per_tile);   // (stepped along from here: a 64-bit division takes longer than a load's issue)
+    int at = (int)(begin - (long)tile0 * wk.per_tile), n0 = tile0 / wk.chunks * 64, chunk = tile0 % wk.chunks;
     for (long i = begin; i < end; ++i) {
-      const int tile = (int)(i / wk.per_tile), k0 = (int)(i - (long)tile * wk.per_tile) * kSlice;
-      const int n0 = tile / wk.chunks * 64, m0 = tile % wk.chunks * N;
+      const int k0 = at * kSlice, m0 = chunk * N;
       if (!tc::mbar_wait_warp(&empty[s], ph ^ 1u)) { ok = false; break; }
       if (tc::elect_one()) {
         uint8_t* dst = smem + s * L::kSlot;
@@ -115,6 +116,10 @@ gated_skinny_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_const
       __syncwarp();
       ++issued;
       if (++s == (uint32_t)L::kSlots) { s = 0; ph ^= 1u; }
+      if (++at == wk.per_tile) {
+        at = 0;
+        if (++chunk == wk.chunks) { chunk = 0; n0 += 64; }
+      }
     }
     if (!ok) {   // loads under way still land here: wait for them, bounded
       if (lane == 0) atomicExch(err_flag, tc::kErrProducerWait);
@@ -236,15 +241,20 @@ gated_shares_kernel(const Work wk, int rows /*of a chunk*/, long ctas, float* __
                     int act) {
   NRS_PDL_PROLOGUE();
   const int tile = blockIdx.x, r = blockIdx.y * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
+  __shared__ int s_shares;   // (one thread's divisions)
+  if (threadIdx.x == 0) {
+    const long first = (long)tile * wk.per_tile;
+    s_shares = (int)(wk.owner(first + wk.per_tile - 1, ctas) - wk.owner(first, ctas)) + 1;
+  }
+  __syncthreads();
   const int row = tile % wk.chunks * rows + r, col = tile / wk.chunks * 64 + c;
   if (r >= rows || row >= m || col >= n) return;
-  const long first = (long)tile * wk.per_tile, c0 = wk.owner(first, ctas), c1 = wk.owner(first + wk.per_tile - 1, ctas);
   const float* src = wk.partial + (long)tile * wk.slots_max * (rows * 128) + r * 128 + c;
   float a = 0.0f, u = 0.0f;
 #pragma unroll 4
-  for (long s = 0; s <= c1 - c0; ++s) {
-    a += src[s * (rows * 128)];
-    u += src[s * (rows * 128) + 64];
+  for (int s = 0; s < s_shares; ++s) {
+    a += src[(long)s * (rows * 128)];
+    u += src[(long)s * (rows * 128) + 64];
   }
   const size_t at = (size_t)row * n + col;
   if (pre_gate) { pre_gate[at] = a; pre_up[at] = u; }

@@ -89,7 +89,8 @@ pub fn batchnorm2d(x: &N, gamma: &N, beta: &N, running_mean: &N, running_var: &N
     resident(out, vec![x.clone(), gamma.clone(), beta.clone()])
 }
 
-/// src/cuda/nn/dropout.rs:32.  The mask is drawn on the device (seeded, `nrs_rng_seed`), not on the host.
+/// src/cuda/nn/dropout.rs:32.  The mask is drawn on the device (seeded, `nrs_rng_seed`), not on the host, and again in the
+/// backward pass instead of being stored.
 pub fn dropout(input: &N, p: f32, training: bool) -> N {
     if !training { return input.clone(); }
     let mut out = std::ptr::null_mut();
@@ -103,6 +104,46 @@ pub fn dropout2d(input: &N, p: f32, training: bool) -> N {
     let mut out = std::ptr::null_mut();
     check(unsafe { sys::nrs_op_dropout2d(handle(input, "cuda dropout2d: input"), p, 1, std::ptr::null_mut(), &mut out) });
     resident(out, vec![input.clone()])
+}
+
+/// residual + dropout(input) in one pass (no reference counterpart).
+pub fn dropout_add(input: &N, residual: &N, p: f32, training: bool) -> N {
+    let mut out = std::ptr::null_mut();
+    check(unsafe {
+        sys::nrs_op_dropout_add(handle(input, "cuda dropout_add: input"), handle(residual, "cuda dropout_add: residual"), p, training as i32,
+                                &mut out)
+    });
+    resident(out, vec![input.clone(), residual.clone()])
+}
+
+/// act(x w_gate) * (x w_up) of a gated feed-forward layer (no reference counterpart; act: `sys::NRS_ACT_*`).
+pub fn gated_linear(x: &N, w_gate: &N, w_up: &N, act: i32) -> N {
+    let mut out = std::ptr::null_mut();
+    check(unsafe {
+        sys::nrs_op_gated_linear(handle(x, "cuda gated linear: input"), handle(w_gate, "cuda gated linear: gate"),
+                                 handle(w_up, "cuda gated linear: up"), act, &mut out)
+    });
+    resident(out, vec![x.clone(), w_gate.clone(), w_up.clone()])
+}
+
+/// RMS norms and position rotations of query and key heads in one pass (no reference counterpart).  The table
+/// (`rotary_table`) is made once.
+pub struct HeadNorm { pub gamma_q: N, pub gamma_k: N, pub table: N, pub interleaved: bool, pub eps: f32 }
+impl HeadNorm {
+    pub fn rotary_table(rot_dim: usize, max_len: usize, base: f32) -> N {
+        let mut out = std::ptr::null_mut();
+        check(unsafe { sys::nrs_rotary_new(ctx(), rot_dim as i64, max_len as i64, base, &mut out) });
+        resident(out, vec![])
+    }
+    pub fn forward(&self, q: &N, k: &N, heads_q: usize, heads_k: usize) -> (N, N) {
+        let (mut oq, mut ok) = (std::ptr::null_mut(), std::ptr::null_mut());
+        check(unsafe {
+            sys::nrs_op_qk_norm_rotary(handle(q, "cuda qk norm: queries"), handle(k, "cuda qk norm: keys"), handle(&self.gamma_q, "cuda qk norm: gamma_q"),
+                                       handle(&self.gamma_k, "cuda qk norm: gamma_k"), handle(&self.table, "cuda qk norm: table"), std::ptr::null(),
+                                       heads_q as i64, heads_k as i64, self.interleaved as i32, self.eps, &mut oq, &mut ok)
+        });
+        (resident(oq, vec![q.clone(), self.gamma_q.clone(), self.table.clone()]), resident(ok, vec![k.clone(), self.gamma_k.clone(), self.table.clone()]))
+    }
 }
 
 /// src/cuda/nn/embedding.rs:35-100.
@@ -128,6 +169,18 @@ impl Embedding {
         check(unsafe {
             sys::nrs_op_embedding_batch(handle(&self.weight, "cuda embedding: weight"), idx.as_ptr(), batch_indices.len() as i64,
                                         seq as i64, &mut out)
+        });
+        resident(out, vec![self.weight.clone()])
+    }
+    /// `forward_batch` with the rows times `scale` and the table's gradient from sorted tokens (no reference counterpart).
+    pub fn forward_batch_scaled(&self, batch_indices: &[Vec<usize>], scale: f32) -> N {
+        let seq = batch_indices.first().map_or(0, |r| r.len());
+        let idx: Vec<i32> = batch_indices.iter().flatten().map(|&i| i as i32).collect();
+        assert_eq!(idx.len(), batch_indices.len() * seq, "embedding: ragged batch");
+        let mut out = std::ptr::null_mut();
+        check(unsafe {
+            sys::nrs_op_embedding_scaled(handle(&self.weight, "cuda embedding: weight"), idx.as_ptr(), batch_indices.len() as i64, seq as i64,
+                                         scale, &mut out)
         });
         resident(out, vec![self.weight.clone()])
     }
