@@ -139,8 +139,10 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {   // inclusive
 __global__ void __launch_bounds__(kSortThreads, 1)
 embed_sort_kernel(const int32_t* __restrict__ idx, const Plan p, const Work w) {
   NRS_PDL_PROLOGUE();
-  extern __shared__ int counts[];                  // [warp][range] tokens of each row in the warp's stretch, then where its next goes
-  __shared__ int s_below[kSortWarps], s_scan[kSortWarps];
+  // (All of it dynamic: whether a launch has to ask for more than the default is judged by that size alone.)
+  extern __shared__ int s_below[];                 // [warp]
+  int* const s_scan = s_below + kSortWarps;        // [warp]
+  int* const counts = s_scan + kSortWarps;         // [warp][range] tokens of each row in the warp's stretch, then where its next goes
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int lo = blockIdx.x * p.range, hi = min(p.vocab, lo + p.range), rows = hi - lo;
   int* const mine = counts + warp * p.range;
@@ -463,7 +465,7 @@ int nrs_embedding_sorted_bwd(nrs_ctx* ctx, const float* g, const int32_t* idx, f
   NRS_REQUIRE(ctx, (long)p.pieces * p.slabs + vocab <= 0x7fffffffL, NRS_ERR_SHAPE, "%s: %d tokens of %d features are too many for one call", __func__, tokens, dim);
   NrsDeviceGuard on(ctx);
   const bool vec = dim % 4 == 0 && (((uintptr_t)g | (uintptr_t)dweight) & 15) == 0;
-  const size_t smem = sizeof(int) * kSortWarps * p.range;
+  const size_t smem = sizeof(int) * kSortWarps * (p.range + 2);
   static NrsSmemAttr attr;
   NRS_ENSURE_SMEM(ctx, attr, embed_sort_kernel, smem);
   NRS_PDL_LAUNCH(embed_sort_kernel, (vocab + p.range - 1) / p.range, kSortThreads, smem, ctx->stream, idx, p, w);

@@ -2,6 +2,9 @@
 token to many, runs that cross blocks, ids outside the vocabulary, odd widths and addresses, captured calls, the node and
 the trainer's layer."""
 import ctypes as C
+import pathlib
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -74,6 +77,27 @@ def test_gradient(gpu_ctx, case):
     got = backward(gpu_ctx, g, ids, vocab, scale, old, shift)
     assert (np.abs(got - (want * s + old)) <= bound + U * 1.001 * np.abs(want * s + old)).all()
     assert np.array_equal(got[terms == 0], old[terms == 0])
+
+
+# A block's counts are 128 bytes a row of its share of the vocabulary: on 148 SMs they pass 48 KB, beyond which a launch has to
+# ask for its shared memory, in this range.  Each in a process of its own: one larger table asks for all that follow.
+@pytest.mark.parametrize("vocab", [56536, 56537, 56700, 56832, 56833])
+def test_vocabularies_around_the_default_shared_memory(vocab):
+    code = f"""
+import ctypes as C
+import numpy as np
+from neuralrs_b200 import cuda
+from tests.test_gpu_embedding_sorted import backward
+rng = np.random.default_rng({vocab})
+ids, g = rng.integers(0, {vocab}, 500), rng.standard_normal((500, 8)).astype(np.float32)
+want = np.zeros(({vocab}, 8))
+np.add.at(want, ids, g.astype(np.float64))
+got = backward(cuda.Context(0), g, ids, {vocab}, 1.0)
+assert np.abs(got - want).max() < 1e-5       # (a few values below 5 a row, each addition off by 2^-24 of them)
+assert (got[np.setdiff1d(np.arange({vocab}), ids)] == 0).all()
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=pathlib.Path(__file__).parent.parent, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_no_tokens(gpu_ctx):
