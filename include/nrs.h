@@ -180,9 +180,12 @@ int nrs_bmm(nrs_ctx* ctx, int trans_a, int trans_b, int batch, int m, int n, int
  * both projections, the activation (any nrs_act; NONE: a product of two projections) and the product in one kernel.
  * pre_gate, pre_up (both or neither): [m,n], the projections, which the backward pass reads.
  * Backward: dx (+)=, and dw_gate, dw_up (+)= (both or neither); dx and the pair may be NULL.
- * 3xTF32 mode: from 16 rows and n, k >= 32 on, f16 pairs in accumulation chains of 256 values, added up in f32: the error of
- * an f32 product.  Fewer rows, and smaller layers: f32.  The other modes: as nrs_gemm of each product.  Like nrs_gemm, the
- * calls use scratch of the context: graphs captured on one context are replayed one after the other. */
+ * 3xTF32 mode, with the error of an f32 product.  Forward: up to 4 rows, and small layers of up to 15, in f32; the
+ * others up to 32 rows, and up to 128 where k >= 256, three TF32 products of operands split in two, summed in f32 every 32
+ * values (n, k multiples of 4 and 16-byte addresses); else, and backward, f16 pairs in accumulation chains of 256 values, added
+ * up in f32, from 16 rows and n, k >= 32 on; what is left in f32.  The other modes: as nrs_gemm of each product (forward, up
+ * to 15 rows: f32).  Like nrs_gemm, the calls use scratch of the context: graphs captured on one context are replayed one
+ * after the other. */
 int nrs_gated_linear_fwd(nrs_ctx* ctx, const float* x, const float* w_gate, const float* w_up, float* h, float* pre_gate,
                          float* pre_up, int m, int n, int k, int act);
 int nrs_gated_linear_bwd(nrs_ctx* ctx, const float* x, const float* w_gate, const float* w_up, const float* pre_gate,
