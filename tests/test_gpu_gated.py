@@ -185,6 +185,57 @@ def test_infinities_stay_in_their_row(gpu_ctx, shape):
     assert not np.isfinite(got["dwg"]).all()
 
 
+# The form that reads the weights as they lie (16 to 32 rows, and to 128 from 256 values of k on; 16, 32, 64 and 128 columns).
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(16, 64, 64), (20, 96, 100), (50, 128, 256), (128, 64, 300)], ids=lambda s: "x".join(map(str, s)))
+def test_infinities_stay_in_their_row_of_few(gpu_ctx, shape):
+    m, n, k = shape
+    x, wg, wu, dh = inputs(np.random.default_rng(7), m, n, k)
+    x[1, 5], x[3, 0] = np.inf, np.nan
+    with np.errstate(all="ignore"):
+        got = run(gpu_ctx, x, wg, wu, dh, SILU, keep=False)["h"]
+    assert not np.isfinite(got[1]).all() and not np.isfinite(got[3]).any()
+    rest = np.setdiff1d(np.arange(m), [1, 3])
+    want = formulas(*(v.astype(np.float64) for v in (x[rest], wg, wu)), SILU, dh[rest].astype(np.float64))
+    assert rel_l2(got[rest], want["h"]) < 1e-5
+    x[1, 5], x[3, 0] = 1.0, 1.0
+    wg[2, 9], wu[2, 9] = np.inf, np.inf                   # a column of the weights
+    with np.errstate(all="ignore"):
+        got = run(gpu_ctx, x, wg, wu, dh, SILU, keep=False)["h"]
+    rest = np.setdiff1d(np.arange(n), [9])
+    want = formulas(*(v.astype(np.float64) for v in (x, wg[:, rest], wu[:, rest])), SILU, dh[:, rest].astype(np.float64))
+    assert rel_l2(got[:, rest], want["h"]) < 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [16, 100])
+def test_captured_calls_of_few_rows_replay(gpu_ctx, m):
+    import torch
+    s, l, ctx = torch.cuda.Stream(), _lib.lib(), cuda.Context(0)
+    ctx.set_stream(s.cuda_stream)
+    n, k = 192, 512
+    with torch.cuda.stream(s):
+        x, wg, wu, h = (torch.randn(*d, device="cuda") for d in ((m, k), (k, n), (k, n), (m, n)))
+        f = lambda: _lib.check(ctx.h, l.nrs_gated_linear_fwd(ctx.h, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), None, None, m, n, k, SILU))
+        f()
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            f()
+        # scratch that grows after the capture leaves the graph its own
+        big = torch.randn(m, 4096, device="cuda"), torch.randn(4096, 2000, device="cuda"), torch.empty(m, 2000, device="cuda")
+        _lib.check(ctx.h, l.nrs_gated_linear_fwd(ctx.h, big[0].data_ptr(), big[1].data_ptr(), big[1].data_ptr(), big[2].data_ptr(), None, None, m, 2000, 4096, SILU))
+        for _ in range(2):
+            x.copy_(torch.randn(m, k, device="cuda"))
+            h.fill_(float("nan"))
+            graph.replay()
+            s.synchronize()
+            a, u = (x.double() @ w.double() for w in (wg, wu))
+            want = torch.nn.functional.silu(a) * u
+            assert ((h.double() - want).norm() / want.norm()).item() < 1e-5
+    del graph
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m", [4, 300])
 def test_captured_calls_replay(gpu_ctx, m):
