@@ -183,7 +183,8 @@ int nrs_bmm(nrs_ctx* ctx, int trans_a, int trans_b, int batch, int m, int n, int
  * 3xTF32 mode, with the error of an f32 product.  Forward: up to 4 rows, and small layers of up to 15, in f32; the
  * others up to 32 rows, and up to 128 where k >= 256, three TF32 products of operands split in two, summed in f32 every 32
  * values (n, k multiples of 4 and 16-byte addresses); else, and backward, f16 pairs in accumulation chains of 256 values, added
- * up in f32, from 16 rows and n, k >= 32 on; what is left in f32.  The other modes: as nrs_gemm of each product (forward, up
+ * up in f32, from 16 rows and n, k >= 32 on, every matrix under an exponent of its own (of the two products that dx adds up, the
+ * larger one's); what is left in f32.  The other modes: as nrs_gemm of each product (forward, up
  * to 15 rows: f32).  Like nrs_gemm, the calls use scratch of the context: graphs captured on one context are replayed one
  * after the other. */
 int nrs_gated_linear_fwd(nrs_ctx* ctx, const float* x, const float* w_gate, const float* w_up, float* h, float* pre_gate,

@@ -106,17 +106,17 @@ void nrs_range_drop(nrs_ctx* ctx, const void* p) {
   nrs_range_free(ctx, it->second);
   ctx->ranges.erase(it);
 }
-int nrs_range_renew(nrs_ctx* ctx, const void* p, NrsRange** out) {
+int nrs_range_renew(nrs_ctx* ctx, const void* p, NrsRange** out, int count) {
   nrs_range_drop(ctx, p);
-  const int st = nrs_range_new(ctx, out);
+  const int st = nrs_range_new(ctx, out, count);
   if (st == NRS_OK) ctx->ranges[p] = *out;
   return st;
 }
-int nrs_range_new(nrs_ctx* ctx, NrsRange** out) {
+int nrs_range_new(nrs_ctx* ctx, NrsRange** out, int count) {
   NrsRangePool& pool = ctx->range_pool;
   *out = nullptr;
   constexpr size_t kBytes = NrsRangePool::kPerPage * sizeof(NrsRange);
-  if (pool.captured_left == 0) {   // (ahead of the first capture: the driver may refuse memory during one)
+  if (pool.captured_left < count) {   // (ahead of the first capture: the driver may refuse memory during one)
     void* mem = nullptr;
     const int st = nrs_alloc(ctx, NrsRangePool::kCaptured * sizeof(NrsRange), 0, &mem);
     if (st != NRS_OK) return st;
@@ -126,12 +126,13 @@ int nrs_range_new(nrs_ctx* ctx, NrsRange** out) {
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
   NRS_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capturing));
   if (capturing != cudaStreamCaptureStatusNone) {
-    *out = pool.captured++;
-    --pool.captured_left;
-    NRS_CUDA(ctx, cudaMemsetAsync(*out, 0, sizeof(NrsRange), ctx->stream));
+    *out = pool.captured;
+    pool.captured += count;
+    pool.captured_left -= count;
+    NRS_CUDA(ctx, cudaMemsetAsync(*out, 0, count * sizeof(NrsRange), ctx->stream));
     return NRS_OK;
   }
-  if (pool.pages.empty() || pool.pages[pool.current].used == NrsRangePool::kPerPage) {
+  if (pool.pages.empty() || pool.pages[pool.current].used + count > NrsRangePool::kPerPage) {
     size_t next = 0;
     while (next < pool.pages.size() && pool.pages[next].live > 0) ++next;
     if (next == pool.pages.size()) {
@@ -146,7 +147,8 @@ int nrs_range_new(nrs_ctx* ctx, NrsRange** out) {
     pool.current = next;
   }
   NrsRangePool::Page& pg = pool.pages[pool.current];
-  *out = pg.mem + pg.used++;
+  *out = pg.mem + pg.used;
+  pg.used += count;
   ++pg.live;
   return NRS_OK;
 }

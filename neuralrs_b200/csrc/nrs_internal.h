@@ -312,9 +312,10 @@ int nrs_ws_slot(nrs_ctx* ctx, int slot, size_t bytes, void** out);
 int nrs_ws_planes(nrs_ctx* ctx, int slot, size_t values, bool split, void** hi, void** lo);
 // A new range, all zero, for what is written to `p` next; it belongs to the address until that is renewed, dropped or
 // freed (nrs_free).
-int nrs_range_renew(nrs_ctx* ctx, const void* p, NrsRange** out);
+// (`count`: of matrices side by side in the planes, their ranges one behind the other)
+int nrs_range_renew(nrs_ctx* ctx, const void* p, NrsRange** out, int count = 1);
 // The same without an address: the caller gives it back.
-int nrs_range_new(nrs_ctx* ctx, NrsRange** out);
+int nrs_range_new(nrs_ctx* ctx, NrsRange** out, int count = 1);
 void nrs_range_free(nrs_ctx* ctx, NrsRange* r);
 void nrs_range_drop(nrs_ctx* ctx, const void* p);
 inline NrsRange* nrs_range_of(const nrs_ctx* ctx, const void* p) {

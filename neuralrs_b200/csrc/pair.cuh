@@ -26,8 +26,9 @@ __device__ __forceinline__ float scale_of(float bound) { return pow2(scale_exp(b
 struct Unscale {
   float a, a_lo, b;
   bool halves;   // nearly never: one factor does
-  __device__ __forceinline__ Unscale(float bound_a, float bound_b) {
-    const int e = -(scale_exp(bound_a) + scale_exp(bound_b));
+  __device__ __forceinline__ Unscale(float bound_a, float bound_b) : Unscale(scale_exp(bound_a) + scale_exp(bound_b)) {}
+  __device__ __forceinline__ explicit Unscale(int exponents) {
+    const int e = -exponents;
     halves = e < -115 || e > 127;
     const int first = halves ? e / 2 : e;
     a = pow2(first);

@@ -12,6 +12,11 @@
 // by side in one row.  The forward product reads the weights' planes with k across the rows, dx along them, the weight
 // gradients x and da|du across: nothing is transposed (staging 2048 x 5504 weights transposed took 112 us, as they are 36).
 // All of a pass's operands are measured by one launch and written by another.
+//
+// Every matrix has an exponent of its own, also where two lie side by side: a and u, dWg and dWu are results apart, and what is
+// small in one of them is not to lose bits to the other.  dx adds da Wg^T and du Wu^T in one accumulator, so there the
+// exponents of Wg and Wu are chosen such that both products carry the same one, that of the larger product: the other gives
+// up only what lies below the sum's own bits.
 #include "gated.h"
 #include "tc_mainloop.cuh"
 
@@ -34,6 +39,7 @@ struct GatedPolicy {
   float* pre[2];         // forward: a, u, or null
   int M, N;              // of the output as it is stored (weights: of one matrix)
   int ld;                // n, padded: columns of one of the two matrices side by side
+  const NrsRange *ra, *rb;   // of A's and B's matrices
   int act, accumulate;
   bool vec;              // rows of the outputs start on 16 bytes
   bool independent;      // of the kernel launched before it
@@ -71,6 +77,12 @@ struct GatedPolicy {
     }
   }
   __device__ __forceinline__ float out_bound(float, float, int) const { return 0.0f; }
+  // Both operands' exponents in the sums that belong to matrix `mat`; and which one a warp's i-th block, at column n, belongs to.
+  __device__ __forceinline__ int exponents(int mat) const {
+    if (P == kInput) return min(pr::scale_exp(ra[0].top) + pr::scale_exp(rb[0].top), pr::scale_exp(ra[1].top) + pr::scale_exp(rb[1].top));
+    return pr::scale_exp(ra[0].top) + pr::scale_exp(rb[mat].top);
+  }
+  __device__ __forceinline__ bool second(int i, int n) const { return P == kForward ? i == 1 : P == kWeights && n >= ld; }
   __device__ __forceinline__ int row(int, int, int) const { return 0; }
   template <int W>
   __device__ __forceinline__ int fetch(int, int, bool) const { return 0; }
@@ -145,7 +157,8 @@ struct Job {
   const float* src;
   const float *a, *u;
   __half *hi, *lo;
-  NrsRange* range;
+  NrsRange* range;          // of da and du: two
+  const NrsRange *other, *with, *other_with;   // of a weight in dx's sum: the other weight's, and those of what the two are multiplied by
   int rows, cols, pad;      // pad: a row's values in the planes, cols rounded up to 64
   long ld;                  // values between rows of the planes
   unsigned first, blocks;   // of the launch
@@ -180,23 +193,25 @@ __device__ __forceinline__ const Job& job_of(const Jobs& jobs) {
   return jobs.j[which];
 }
 
-// The largest magnitude of each tensor into its range.  Of da and du: of dh u, times 1.13, which no activation's slope exceeds,
-// and of dh a, which no activation exceeds; without their exponentials this is a pass at memory speed.
+// The largest magnitude of each tensor into its range.  Of da and du themselves, exponentials and all: a bound from dh u and
+// dh a is cheaper, but a gate far to the left, which passes nothing on, would set the exponent for all the others.
 __global__ void __launch_bounds__(256, 3) gated_measure_kernel(const Jobs jobs) {
   NRS_PDL_PROLOGUE();
   const Job& q = job_of(jobs);
   const size_t count = (size_t)q.rows * q.cols, units = q.whole ? count / 8 : 0, step = (size_t)q.blocks * 256;   // (whole: 16-byte accesses)
   const bool grads = q.a != nullptr;
-  uint32_t top = 0;
+  uint32_t top = 0, top_u = 0;
   auto see = [&](float (&g)[8], float (&a)[8], float (&u)[8]) {
     if (grads) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        u[i] *= 1.13f * g[i];
-        a[i] *= g[i];
+        float f, d;
+        gated::act_both(a[i], jobs.act, f, d);
+        a[i] = g[i] * u[i] * d;
+        u[i] = g[i] * f;
       }
-      top = pr::seen_all(top, u);
       top = pr::seen_all(top, a);
+      top_u = pr::seen_all(top_u, u);
     } else {
       top = pr::seen_all(top, g);
     }
@@ -223,11 +238,13 @@ __global__ void __launch_bounds__(256, 3) gated_measure_kernel(const Jobs jobs) 
     see(g, a, u);
   }
   // (one atomic a block: those of ten thousand warps on one word took longer than the pass)
-  __shared__ uint32_t tops[8];
+  __shared__ uint32_t tops[2][8];
   top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  top_u = __reduce_max_sync(0xffffffffu, top_u);
+  if ((threadIdx.x & 31) == 0) { tops[0][threadIdx.x >> 5] = top; tops[1][threadIdx.x >> 5] = top_u; }
   __syncthreads();
-  if (threadIdx.x < 32) pr::report(q.range, threadIdx.x < 8 ? tops[threadIdx.x] : 0u);
+  const int warp = threadIdx.x >> 5;
+  if (warp < (grads ? 2 : 1)) pr::report(q.range + warp, (threadIdx.x & 31) < 8 ? tops[warp][threadIdx.x & 31] : 0u);
 }
 
 // The pairs, zeros from cols to pad: eight values a thread where rows start on 16 bytes, else 128 values a warp, value by value
@@ -236,8 +253,9 @@ __global__ void __launch_bounds__(256, 4) gated_stage_kernel(const Jobs jobs) {
   NRS_PDL_PROLOGUE();
   const Job& q = job_of(jobs);
   const bool grads = q.a != nullptr;
-  const float bound = q.range->top, scale = pr::scale_of(bound);
-  if (blockIdx.x == q.first && threadIdx.x == 0) q.range->bound = bound;
+  int e = pr::scale_exp(q.range->top);
+  if (q.other) e = min(e, pr::scale_exp(q.other->top) + pr::scale_exp(q.other_with->top) - pr::scale_exp(q.with->top));
+  const float scale = e < -126 ? 0.0f : pr::pow2(e), scale_u = grads ? pr::scale_of(q.range[1].top) : 0.0f;   // (0: nothing of it reaches the sum)
   if (q.vec) {
     const uint32_t units = (uint32_t)q.rows * (uint32_t)(q.pad / 8), step = q.blocks * 256;   // (the launcher checks the range)
     for (uint32_t i = (blockIdx.x - q.first) * 256 + threadIdx.x; i < units; i += step) {
@@ -263,7 +281,7 @@ __global__ void __launch_bounds__(256, 4) gated_stage_kernel(const Jobs jobs) {
         u[k] = g[k] * f;
       }
       put8(q.hi, q.lo, at, a, scale);
-      put8(q.hi, q.lo, at + q.pad, u, scale);
+      put8(q.hi, q.lo, at + q.pad, u, scale_u);
     }
     return;
   }
@@ -293,7 +311,7 @@ __global__ void __launch_bounds__(256, 4) gated_stage_kernel(const Jobs jobs) {
       float f, d;
       gated::act_both(a[k], jobs.act, f, d);
       pr::put(q.hi, q.lo, at + 32 * k, g[k] * u[k] * d, scale);
-      pr::put(q.hi, q.lo, at + q.pad + 32 * k, g[k] * f, scale);
+      pr::put(q.hi, q.lo, at + q.pad + 32 * k, g[k] * f, scale_u);
     }
   }
 }
@@ -302,14 +320,14 @@ int round64(int v) { return (v + 63) / 64 * 64; }
 
 struct Planes {
   void *hi, *lo;
-  NrsRange* range;
+  NrsRange* range;          // one for each matrix in a row
   int pad, ld;              // values of one matrix in a row, and of a row
 };
 int open_planes(nrs_ctx* ctx, int slot, int rows, int cols, int side_by_side, Planes* out) {
   out->pad = round64(cols);
   out->ld = side_by_side * out->pad;
   const int st = nrs_ws_planes(ctx, slot, (size_t)rows * out->ld, true, &out->hi, &out->lo);
-  return st == NRS_OK ? nrs_range_renew(ctx, out->hi, &out->range) : st;
+  return st == NRS_OK ? nrs_range_renew(ctx, out->hi, &out->range, side_by_side) : st;
 }
 bool aligned(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
@@ -320,7 +338,7 @@ void add_job(Jobs* jobs, const float* src, const float* a, const float* u, int r
   Job& q = jobs->j[jobs->count++];
   q.src = src; q.a = a; q.u = u;
   q.hi = (__half*)to.hi + (size_t)mat * to.pad; q.lo = (__half*)to.lo + (size_t)mat * to.pad;
-  q.range = to.range;
+  q.range = to.range + mat;
   q.rows = rows; q.cols = cols; q.pad = to.pad; q.ld = to.ld;
   q.whole = aligned({src, a, u});
   q.vec = q.whole && cols % 4 == 0;
@@ -361,7 +379,7 @@ bool map_mn(CUtensorMap* t, const void* base, const Planes& p, int k, int box_co
 
 // The product of A [rows] and B [cols, padding included]; k: its length (input: of one matrix).
 template <int BN, bool PAIR, Product P>
-int run(nrs_ctx* ctx, const Planes& A, const Planes& B, const GatedPolicy<P>& pol, int rows, int cols, int k, int* splits = nullptr) {
+int run(nrs_ctx* ctx, const Planes& A, const Planes& B, GatedPolicy<P> pol, int rows, int cols, int k, int* splits = nullptr) {
   constexpr int kBCols = PAIR || P == kForward ? BN / 2 : BN;   // of B in one load
   CUtensorMap a[2], b[2];
   bool ok = true;
@@ -371,9 +389,11 @@ int run(nrs_ctx* ctx, const Planes& A, const Planes& B, const GatedPolicy<P>& po
     ok = ok && (P == kInput ? map_k(&b[i], pb, B, k, cols, 2, kBCols) : map_mn(&b[i], pb, B, k, kBCols));
   }
   NRS_REQUIRE(ctx, ok, NRS_ERR_CUDA, "gated layer: cuTensorMapEncodeTiled failed (%d x %d x %d)", rows, cols, k);
+  pol.ra = A.range;
+  pol.rb = B.range;
   const int kb = P == kInput ? 2 * (A.pad / 64) : (k + 63) / 64;
   return tc::launch<BN, 2, PAIR, 64, GatedPolicy<P>>(ctx, a[0], a[1], b[0], b[1], pol, (rows + tc::BM - 1) / tc::BM, cols, 1, kb,
-                                                     tc::Ranges{A.range, B.range, nullptr}, nullptr, nullptr, splits);
+                                                     tc::Ranges{}, nullptr, nullptr, splits);
 }
 
 bool applies(const nrs_ctx* ctx, const Shape& s) {
@@ -423,6 +443,10 @@ int nrs_tc_gated_bwd(nrs_ctx* ctx, const Shape& s, const float* x, const float* 
   if (dx) {
     add_job(&jobs, w_gate, nullptr, nullptr, s.k, s.n, W, 0);
     add_job(&jobs, w_up, nullptr, nullptr, s.k, s.n, W, 1);
+    for (int mat = 0; mat < 2; ++mat) {
+      Job& q = jobs.j[jobs.count - 2 + mat];
+      q.other = W.range + 1 - mat; q.with = D.range + mat; q.other_with = D.range + 1 - mat;
+    }
   }
   st = run_jobs(ctx, jobs);
   if (st != NRS_OK) return st;

@@ -571,7 +571,10 @@ tc_kernel(const __grid_constant__ CUtensorMap tm_a_hi, const __grid_constant__ C
     uint8_t* team_tile = emit_tile + (Policy::kCanEmit ? team * BM * 128 : 0);
     [[maybe_unused]] float out_scale = 1.0f;
     [[maybe_unused]] uint32_t top = 0;
-    [[maybe_unused]] const pr::Unscale unscale(NPLANES == 2 ? rg.a->bound : 1.0f, NPLANES == 2 ? rg.b->bound : 1.0f);
+    [[maybe_unused]] int exponents[2] = {0, 0};   // ShortChains: of each of the matrices that lie side by side
+    if constexpr (ShortChains<Policy>::value) { exponents[0] = pol.exponents(0); exponents[1] = pol.exponents(1); }
+    constexpr bool kRanges = NPLANES == 2 && !ShortChains<Policy>::value;
+    [[maybe_unused]] const pr::Unscale unscale(kRanges ? rg.a->bound : 1.0f, kRanges ? rg.b->bound : 1.0f);
     if constexpr (NPLANES == 2) {
       if (rg.out) {
         const float bound = pol.out_bound(rg.a->top, rg.b->top, lane);
@@ -624,7 +627,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tm_a_hi, const __grid_constant__ C
               tmem_ld_32(acc + (uint32_t)(c * kW), r);
               tmem_ld_32(acc + (uint32_t)(BN + c * kW), r2);
               tmem_ld_wait();
-              unscale.apply(r, r2);
+              pr::Unscale(pol.second(i, n0 + c * kW) ? exponents[1] : exponents[0]).apply(r, r2);
 #pragma unroll
               for (int j = 0; j < kW; ++j) sums[i][j] += __uint_as_float(r[j]);
             }

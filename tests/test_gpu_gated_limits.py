@@ -1,0 +1,117 @@
+"""Gated feed-forward layers at the limits of what they are given: matrices of very different magnitudes side by side, gates far from
+zero.  Against the formulas in 64 bits."""
+import numpy as np
+import pytest
+
+from .conftest import rel_l2
+from .gpu_util import Dev, call
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+GELU, SILU = 2, 3
+
+
+def sigmoid(v):
+    with np.errstate(over="ignore"):
+        return 1 / (1 + np.exp(-v))
+
+
+def act(a, kind):
+    """act(a) and its slope without a cancellation; and the sigmoid's argument."""
+    a = np.asarray(a, np.float64)
+    w = a if kind == SILU else 2 * 0.7978845608 * (a + 0.044715 * a ** 3)
+    dw = 1.0 if kind == SILU else 2 * 0.7978845608 * (1 + 3 * 0.044715 * a * a)
+    s, r = sigmoid(w), sigmoid(-w)                        # (1 - s, to its own last bit)
+    return a * s, s + np.where(s * r > 0, a * (s * r) * dw, 0.0), w
+
+def inputs(rng, m, n, k):
+    s = 1 / np.sqrt(k)
+    return [v.astype(np.float32) for v in (rng.standard_normal((m, k)), rng.standard_normal((k, n)) * s, rng.standard_normal((k, n)) * s, rng.standard_normal((m, n)))]
+
+
+def formulas(x, wg, wu, dh, a, u):
+    """The gradients for projections a and u as they were kept (SiLU)."""
+    x, wg, wu, dh, a, u = (v.astype(np.float64) for v in (x, wg, wu, dh, a, u))
+    f, d, _ = act(a, SILU)
+    da, du = dh * u * d, dh * f
+    return dict(dx=da @ wg.T + du @ wu.T, dwg=x.T @ da, dwu=x.T @ du)
+
+
+def backward(ctx, x, wg, wu, a, u, dh):
+    (m, k), n = x.shape, wg.shape[1]
+    out = [Dev(ctx, np.full_like(v, np.nan)) for v in (x, wg, wu)]
+    call(ctx, "nrs_gated_linear_bwd", *(Dev(ctx, v) for v in (x, wg, wu, a, u, dh)), *out, m, n, k, SILU, 0, 0)
+    return dict(zip(("dx", "dwg", "dwu"), (o.get() for o in out)))
+
+
+# Chains of 256 values of a UMMA's truncated sums, and the operands' two roundings (tests/test_gpu_gated.py counts the same):
+# whatever the other matrix is.
+SHAPES = [(64, 64, 64), (200, 100, 136), (300, 260, 520), (700, 320, 96)]
+LEVELS = [2.0 ** -40, 2.0 ** -90, 2.0 ** 40]
+
+
+@pytest.mark.parametrize("level", LEVELS)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("which", ["gate", "up"])
+def test_a_weight_far_below_the_other(gpu_ctx, which, shape, level):
+    m, n, k = shape
+    x, wg, wu, _ = inputs(np.random.default_rng(m), m, n, k)
+    (wg if which == "gate" else wu)[:] *= np.float32(level)
+    h, a, u = (Dev(gpu_ctx, np.full((m, n), np.nan, np.float32)) for _ in range(3))
+    call(gpu_ctx, "nrs_gated_linear_fwd", Dev(gpu_ctx, x), Dev(gpu_ctx, wg), Dev(gpu_ctx, wu), h, a, u, m, n, k, SILU)
+    for got, w in ((a.get(), wg), (u.get(), wu)):
+        assert rel_l2(got, x.astype(np.float64) @ w) <= 3 * 8 * U
+
+
+@pytest.mark.parametrize("level", LEVELS)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_a_gradient_far_below_the_other(gpu_ctx, shape, level):
+    """A gate whose weights are small: its pre-activations, and so the other matrix's gradient, are as small."""
+    m, n, k = shape
+    x, wg, wu, dh = inputs(np.random.default_rng(m), m, n, k)
+    a, u = ((x.astype(np.float64) @ w).astype(np.float32) for w in (wg, wu))
+    # (dx: both of its terms at the same level, or the gate's alone)
+    for scaled in (wg, wg * np.float32(level)):
+        b = a * np.float32(level)
+        got, want = backward(gpu_ctx, x, scaled, wu, b, u, dh), formulas(x, scaled, wu, dh, b, u)
+        for name in got:
+            assert rel_l2(got[name], want[name]) <= 3 * 8 * U * 1.2, name
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_closed_gates_leave_the_others_their_bits(gpu_ctx, shape):
+    """Gates far to the left pass nothing on, and what they are says nothing about the others' magnitudes."""
+    m, n, k = shape
+    rng = np.random.default_rng(m)
+    x, wg, wu, dh = inputs(rng, m, n, k)
+    a, u = ((x.astype(np.float64) @ w).astype(np.float32) for w in (wg, wu))
+    shut = rng.random((m, n)) < 0.3
+    a[shut] = -1e9
+    u[shut] *= np.float32(2.0 ** 60)
+    got, want = backward(gpu_ctx, x, wg, wu, a, u, dh), formulas(x, wg, wu, dh, a, u)
+    for name in got:
+        assert rel_l2(got[name], want[name]) <= 3 * 8 * U * 1.2, name
+
+
+def test_a_weight_of_zeros(gpu_ctx):
+    m, n, k = 200, 96, 128
+    x, wg, wu, dh = inputs(np.random.default_rng(9), m, n, k)
+    zero = np.zeros_like(wu)
+    a = (x.astype(np.float64) @ wg).astype(np.float32)
+    got, want = backward(gpu_ctx, x, wg, zero, a, np.zeros_like(a), dh), formulas(x, wg, zero, dh, a, np.zeros_like(a))
+    assert (got["dx"] == 0).all() and (got["dwg"] == 0).all()
+    assert rel_l2(got["dwu"], want["dwu"]) <= 3 * 8 * U * 1.2
+
+
+@pytest.mark.parametrize("v", [1e12, 1e20, 1e30])
+@pytest.mark.parametrize("kind", [GELU, SILU])
+def test_values_far_to_the_right(gpu_ctx, kind, v):
+    """Gates of 1e12 and more beside ordinary values in the other matrix; x is the identity."""
+    m, n, k = 200, 64, 224
+    x, wg, wu = np.eye(m, k, dtype=np.float32), np.full((k, n), v, np.float32), np.ones((k, n), np.float32)
+    h = Dev(gpu_ctx, np.full((m, n), np.nan, np.float32))
+    call(gpu_ctx, "nrs_gated_linear_fwd", Dev(gpu_ctx, x), Dev(gpu_ctx, wg), Dev(gpu_ctx, wu), h, None, None, m, n, k, kind)
+    assert (np.abs(h.get() - float(np.float32(v))) <= 16 * U * v).all()
+    a, one, dw = np.full((m, n), v, np.float32), np.ones((m, n), np.float32), [Dev(gpu_ctx, np.full((k, n), np.nan, np.float32)) for _ in range(2)]
+    call(gpu_ctx, "nrs_gated_linear_bwd", Dev(gpu_ctx, x), None, None, Dev(gpu_ctx, a), Dev(gpu_ctx, one), Dev(gpu_ctx, one), None, *dw, m, n, k, kind, 0, 0)
+    assert (np.abs(dw[0].get()[:m] - 1) <= 16 * U).all() and (np.abs(dw[1].get()[:m] - float(np.float32(v))) <= 16 * U * v).all()
