@@ -115,3 +115,70 @@ def test_values_far_to_the_right(gpu_ctx, kind, v):
     a, one, dw = np.full((m, n), v, np.float32), np.ones((m, n), np.float32), [Dev(gpu_ctx, np.full((k, n), np.nan, np.float32)) for _ in range(2)]
     call(gpu_ctx, "nrs_gated_linear_bwd", Dev(gpu_ctx, x), None, None, Dev(gpu_ctx, a), Dev(gpu_ctx, one), Dev(gpu_ctx, one), None, *dw, m, n, k, kind, 0, 0)
     assert (np.abs(dw[0].get()[:m] - 1) <= 16 * U).all() and (np.abs(dw[1].get()[:m] - float(np.float32(v))) <= 16 * U * v).all()
+
+
+FAR = [-8.0, -20.0, -79.0, -81.0, -86.0, -90.0, -1e4, -1e11, -1e12, -1e20, -1e30, -3.4e38, 30.0, 1e4, 1e12, 1e20, 1e30]
+
+
+def allowed(want, w, a):
+    """The sigmoid's argument carries at most five roundings, each of which the exponential makes |w| times as large, and the
+    rest some sixteen; results below f32's normal range (w beyond 87, |a| or its slope in front) may come as zeros."""
+    return (6 * min(abs(w), 90.0) + 24) * U * np.abs(want) + (4e-36 if w < 0 else 0.0) + 2.0 ** -20 * U * abs(a) * (w > 0)
+
+
+@pytest.mark.parametrize("kind", [GELU, SILU])
+@pytest.mark.parametrize("v", FAR)
+@pytest.mark.parametrize("m", [8, 64])                    # f32, and operands as pairs
+def test_slopes_far_from_zero(gpu_ctx, m, v, kind):
+    """x is the identity, so the weights' gradients are the gates' own."""
+    n = 64
+    eye, one, a = np.eye(m, dtype=np.float32), np.ones((m, n), np.float32), np.full((m, n), v, np.float32)
+    dw = [Dev(gpu_ctx, np.full((m, n), np.nan, np.float32)) for _ in range(2)]
+    call(gpu_ctx, "nrs_gated_linear_bwd", Dev(gpu_ctx, eye), None, None, Dev(gpu_ctx, a), Dev(gpu_ctx, one), Dev(gpu_ctx, one), None, *dw, m, n, m, kind, 0, 0)
+    f, d, w = act(np.float32(v), kind)
+    da, du = dw[0].get(), dw[1].get()
+    assert (np.abs(da - d) <= allowed(d, w, 1.0)).all()
+    assert (np.abs(da) <= 1.13).all()                     # what no slope exceeds
+    assert (np.abs(du - f) <= allowed(f, w, v)).all()
+
+
+@pytest.mark.parametrize("kind", [GELU, SILU])
+@pytest.mark.parametrize("v", FAR)
+@pytest.mark.parametrize("m,k", [(1, 64), (4, 64), (16, 64), (64, 256), (200, 224)])   # every form of the forward pass
+def test_values_far_from_zero(gpu_ctx, m, k, v, kind):
+    n = 64
+    x, wg, wu = np.eye(m, k, dtype=np.float32), np.full((k, n), v, np.float32), np.ones((k, n), np.float32)
+    h = Dev(gpu_ctx, np.full((m, n), np.nan, np.float32))
+    call(gpu_ctx, "nrs_gated_linear_fwd", Dev(gpu_ctx, x), Dev(gpu_ctx, wg), Dev(gpu_ctx, wu), h, None, None, m, n, k, kind)
+    f, _, w = act(np.float32(v), kind)
+    # (a pair carries a weight to 2^-22: as an error of w it counts |w| times, as one of the value once)
+    assert (np.abs(h.get() - f) <= allowed(f, w, v) + 8 * U * (1 + min(abs(w), 90.0)) * np.abs(f)).all()
+
+
+@pytest.mark.parametrize("kind", [GELU, SILU])
+def test_nan_and_infinite_gates(gpu_ctx, kind):
+    m = n = 32
+    x, wu = np.eye(m, dtype=np.float32), np.ones((m, n), np.float32)
+    wg = np.ones((m, n), np.float32)
+    wg[0], wg[1] = np.nan, np.inf
+    h = Dev(gpu_ctx, shape=(1, n))
+    for row in (0, 1):
+        call(gpu_ctx, "nrs_gated_linear_fwd", Dev(gpu_ctx, x[row:row + 1]), Dev(gpu_ctx, wg), Dev(gpu_ctx, wu), h, None, None, 1, n, m, kind)
+        assert not np.isfinite(h.get()).any()
+    dw = [Dev(gpu_ctx, shape=(m, n)) for _ in range(2)]
+    a = np.ones((m, n), np.float32)
+    a[3, 5] = np.nan
+    call(gpu_ctx, "nrs_gated_linear_bwd", Dev(gpu_ctx, x), None, None, Dev(gpu_ctx, a), Dev(gpu_ctx, wu), Dev(gpu_ctx, wu), None, *dw, m, n, m, kind, 0, 0)
+    for t in dw:
+        assert np.isnan(t.get()[3, 5])
+
+
+def test_closed_gates_of_the_lowest_value(gpu_ctx):
+    m, n, k = 200, 100, 136
+    rng = np.random.default_rng(m)
+    x, wg, wu, dh = inputs(rng, m, n, k)
+    a, u = ((x.astype(np.float64) @ w).astype(np.float32) for w in (wg, wu))
+    a[rng.random((m, n)) < 0.3] = np.finfo(np.float32).min
+    got, want = backward(gpu_ctx, x, wg, wu, a, u, dh), formulas(x, wg, wu, dh, a, u)
+    for name in got:
+        assert rel_l2(got[name], want[name]) <= 3 * 8 * U * 1.2, name
