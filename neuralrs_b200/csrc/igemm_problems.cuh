@@ -14,6 +14,7 @@
 // tested on a CPU, without a GPU.
 #pragma once
 
+#include <cmath>
 #include <cstddef>
 #include <cstdint>
 
@@ -50,16 +51,15 @@ struct NrsFastDiv {
 // (vgelu / gelu_grad, src/cuda/graph/gelu.rs:12-32), through the identity 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2u)): one
 // exponential and one division where tanhf takes two divergent paths, and
 // no cancellation in 1 + tanh for negative x.
-NRS_HD float nrs_gelu_e(float xi) {   // exp(-2u), kept finite
-  const float u2 = -1.5957691216f * (xi + 0.044715f * xi * xi * xi);
-  return expf(u2 < 80.0f ? u2 : 80.0f);
-}
-NRS_HD float nrs_gelu_f(float xi) { return xi / (1.0f + nrs_gelu_e(xi)); }
+NRS_HD float nrs_gelu_u2(float xi) { return -1.5957691216f * (xi + 0.044715f * xi * xi * xi); }   // -2u
+NRS_HD float nrs_gelu_f(float xi) { return xi / (1.0f + expf(nrs_gelu_u2(xi))); }   // (an infinite exponential leaves 0)
+// (Far out the second term is 0, but its factors leave f32's range: they are held at +-11, the exponential below infinity.)
 NRS_HD float nrs_gelu_d(float xi) {
-  const float e = nrs_gelu_e(xi);
+  const float u2 = nrs_gelu_u2(xi), e = expf(u2 > 88.0f ? 88.0f : u2);   // (NaN stays)
   const float s = 1.0f / (1.0f + e);                                     // 0.5 (1 + tanh(u)); 1 - s = e s
-  const float du2 = 1.5957691216f * (1.0f + 3.0f * 0.044715f * xi * xi);   // 2 du/dx
-  return s + xi * s * (e * s) * du2;
+  const float x = fminf(fmaxf(xi, -11.0f), 11.0f);
+  const float du2 = 1.5957691216f * (1.0f + 3.0f * 0.044715f * x * x);   // 2 du/dx
+  return s + x * s * (e * s) * du2;
 }
 NRS_HD float nrs_apply_act(float v, int act) {
   if (act == 1) return v > 0.0f ? v : 0.0f;
