@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? kBlocksBwd : kBlocksFwd) head_
       float sq = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) sq += A[k][j] * A[k][j] + B[k][j] * B[k][j];
-      const float rstd = rsqrtf(row_sum<L>(sq) * a.inv_d + a.eps);
+      const float root = rsqrtf(row_sum<L>(sq) * a.inv_d + a.eps), rstd = r < rows ? root : 0.0f;   // (past the end, without an eps: no 0 * inf into dgamma)
       if (!BWD) {
         float* y = s.y + (size_t)t[k] * s.ld_y + h[k] * a.d;
 #pragma unroll
