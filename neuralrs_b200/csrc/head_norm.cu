@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, BWD ? kBlocksBwd : kBlocksFwd) head_
       float sq = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) sq += A[k][j] * A[k][j] + B[k][j] * B[k][j];
-      const float root = rsqrtf(row_sum<L>(sq) * a.inv_d + a.eps), rstd = r < rows ? root : 0.0f;   // (past the end, without an eps: no 0 * inf into dgamma)
+      const float root = rsqrtf(row_sum<L>(sq) * a.inv_d + a.eps), rstd = r < rows && (!BWD || p[k] >= 0) ? root : 0.0f;   // (past the end, without an eps: no 0 * inf into dgamma)
       if (!BWD) {
         float* y = s.y + (size_t)t[k] * s.ld_y + h[k] * a.d;
 #pragma unroll
@@ -172,9 +172,9 @@ __global__ void __launch_bounds__(kThreads, BWD ? kBlocksBwd : kBlocksFwd) head_
       } else {
         float(&ga)[4] = GA[BWD ? k : 0];
         float(&gb)[4] = GB[BWD ? k : 0];
-        if (p[k] < 0) {
+        if (p[k] < 0) {   // (whatever the row holds: the normed values below are 0, too)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) ga[j] = gb[j] = 0.0f;
+          for (int j = 0; j < 4; ++j) A[k][j] = B[k][j] = ga[j] = gb[j] = 0.0f;
         }
         if (turns) rotate<INTER>(ga, gb, t0[k], t1[k], true);
         float dot = 0.0f;
@@ -258,8 +258,11 @@ __global__ void __launch_bounds__(kThreads) head_norm_any_kernel(const Args a, i
       e = v[first(i)];
       f = i < half ? v[second(i)] : 0.0f;
       if (back && i < half) turn(e, f, row[2 * i], -row[2 * i + 1]);
-      if (back && p < 0) e = f = 0.0f;
     };
+    if (BWD && p < 0) {                 // nothing of the row counts, whatever it holds
+      for (int c = lane; y && !a.accumulate && c < a.d; c += 32) y[c] = 0.0f;
+      continue;
+    }
     float sq = 0.0f;
     for (int c = lane; c < a.d; c += 32) sq += x[c] * x[c];
     const float rstd = rsqrtf(row_sum<32>(sq) * a.inv_d + a.eps);
