@@ -491,7 +491,8 @@ class nn:
             self.gamma_q, self.gamma_k, self.rotary, self.interleaved, self.eps = gamma_q, gamma_k, rotary, interleaved, eps
 
         def parameters(self):
-            return [g for g in (self.gamma_q, self.gamma_k) if g is not None]
+            both = [g for g in (self.gamma_q, self.gamma_k) if g is not None]
+            return both[:1] if len(both) == 2 and both[0] is both[1] else both   # (one weight of both sides: one parameter)
 
         def _handles(self):
             return [n.h if n is not None else None for n in (self.gamma_q, self.gamma_k, self.rotary.table if self.rotary else None)]
@@ -515,7 +516,7 @@ class nn:
             self.d_model, self.num_heads, self.causal, self.head_norm = d_model, num_heads, causal, head_norm
 
         def parameters(self):
-            return [self.w_q, self.w_k, self.w_v, self.w_o]
+            return [self.w_q, self.w_k, self.w_v, self.w_o] + (self.head_norm.parameters() if self.head_norm is not None else [])
 
         def forward_batch(self, x: Node) -> Node:
             h = VP()
