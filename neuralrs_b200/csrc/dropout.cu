@@ -10,6 +10,7 @@
 // shape; a caller that wants the reference's own masks passes them to nrs_mask_mul instead.
 #include <cmath>
 
+#include "igemm_problems.cuh"
 #include "nrs_internal.h"
 #include "philox.cuh"
 
@@ -91,20 +92,42 @@ mask_mul_kernel(const float* __restrict__ a, const float* __restrict__ mask, flo
 // upper half all threads of a launch share (a call that crosses 2^32 takes two launches), which spares two of twenty
 // products, 178 with the form without a second operand compiled apart (39 registers, six blocks an SM); 165 with a toy
 // generator in its place.  The copy rate allows 166.
-//   FOURS: hw == 1, a block's four words serve four neighbouring elements; otherwise element i takes mask value i / hw
-//   VEC:   16-byte accesses (FOURS: aligned tensors; planes: hw a multiple of 4 too, so that a vector has one mask value)
 struct Draw {
   uint64_t seed, first;
   uint32_t last;           // words up to here are dropped ones
   float dropped, kept;     // their factor, and the others'
   __device__ __forceinline__ float factor(uint32_t word) const { return word <= last ? dropped : kept; }
 };
-template <bool FOURS, bool VEC, bool ADD>
+constexpr int kUnroll = 4;   // vectors of a thread under way together
+
+// Four elements from 4 * b on, of `total`; VEC: 16-byte accesses to all that are whole.
+template <bool VEC>
+__device__ __forceinline__ float4 load_four(const float* a, size_t b, size_t total) {
+  if (VEC && 4 * b + 4 <= total) return reinterpret_cast<const float4*>(a)[b];
+  float e[4] = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (4 * b + j < total) e[j] = a[4 * b + j];
+  return make_float4(e[0], e[1], e[2], e[3]);
+}
+template <bool VEC>
+__device__ __forceinline__ void store_four(float* out, size_t b, size_t total, float4 y) {
+  if (VEC && 4 * b + 4 <= total) {
+    reinterpret_cast<float4*>(out)[b] = y;
+  } else {
+    const float e[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (4 * b + j < total) out[4 * b + j] = e[j];
+  }
+}
+
+// A value per element: a block's four words serve four neighbouring elements.
+template <bool VEC, bool ADD>
 __global__ void __launch_bounds__(kThreads)
-dropout_kernel(const float* a, const float* residual, float* out, size_t total, size_t hw, const Draw draw, int accumulate) {
+dropout_kernel(const float* a, const float* residual, float* out, size_t total, const Draw draw, int accumulate) {
   NRS_PDL_PROLOGUE();
-  constexpr int kUnroll = 4;   // vectors of a thread under way together
-  const size_t groups = (FOURS || VEC) ? (total + 3) / 4 : total;
+  const size_t groups = (total + 3) / 4;
   const float* add = ADD ? (accumulate ? out : residual) : nullptr;
   for (size_t base = (size_t)blockIdx.x * (kThreads * kUnroll) + threadIdx.x; base < groups; base += (size_t)gridDim.x * (kThreads * kUnroll)) {
     float4 v[kUnroll], r[kUnroll];
@@ -113,52 +136,73 @@ dropout_kernel(const float* a, const float* residual, float* out, size_t total, 
       const size_t b = base + (size_t)u * kThreads;
       v[u] = r[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (b >= groups) continue;
-      if (VEC && 4 * b + 4 <= total) {
-        v[u] = reinterpret_cast<const float4*>(a)[b];
-        if (ADD) r[u] = reinterpret_cast<const float4*>(add)[b];
-      } else if (FOURS) {
-        float e[4] = {}, f[4] = {};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (4 * b + j < total) { e[j] = a[4 * b + j]; if (ADD) f[j] = add[4 * b + j]; }
-        v[u] = make_float4(e[0], e[1], e[2], e[3]);
-        r[u] = make_float4(f[0], f[1], f[2], f[3]);
-      } else {
-        v[u].x = a[b];
-        if (ADD) r[u].x = add[b];
-      }
+      v[u] = load_four<VEC>(a, b, total);
+      if (ADD) r[u] = load_four<VEC>(add, b, total);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const size_t b = base + (size_t)u * kThreads;
       if (b >= groups) continue;
       uint32_t w[4];
-      float4 m;
-      if (FOURS) {
-        nrs_rng::block(draw.seed, (draw.first >> 32 << 32) | (uint32_t)((uint32_t)draw.first + (uint32_t)b), w);
-        m = make_float4(draw.factor(w[0]), draw.factor(w[1]), draw.factor(w[2]), draw.factor(w[3]));
-      } else {
-        const size_t at = VEC ? 4 * b : b, i = (at | hw) >> 32 ? at / hw : (size_t)((uint32_t)at / (uint32_t)hw);
-        nrs_rng::block(draw.seed, draw.first + i / 4, w);
-        const uint32_t k = (uint32_t)i & 3u;
-        const float one = draw.factor(k < 2 ? (k == 0 ? w[0] : w[1]) : (k == 2 ? w[2] : w[3]));
-        m = make_float4(one, one, one, one);
-      }
+      nrs_rng::block(draw.seed, (draw.first >> 32 << 32) | (uint32_t)((uint32_t)draw.first + (uint32_t)b), w);
+      const float4 m = make_float4(draw.factor(w[0]), draw.factor(w[1]), draw.factor(w[2]), draw.factor(w[3]));
       float4 y = make_float4(v[u].x * m.x, v[u].y * m.y, v[u].z * m.z, v[u].w * m.w);
       if (ADD) {   // rounded once, as mask_mul_kernel does (but for the rest of a length that is no multiple of four)
         if (VEC && 4 * b + 4 > total) y = make_float4(__fadd_rn(r[u].x, y.x), __fadd_rn(r[u].y, y.y), __fadd_rn(r[u].z, y.z), 0.0f);
         else y = make_float4(fmaf(v[u].x, m.x, r[u].x), fmaf(v[u].y, m.y, r[u].y), fmaf(v[u].z, m.z, r[u].z), fmaf(v[u].w, m.w, r[u].w));
       }
-      if (VEC && 4 * b + 4 <= total) {
-        reinterpret_cast<float4*>(out)[b] = y;
-      } else if (FOURS) {
-        const float e[4] = {y.x, y.y, y.z, y.w};
+      store_four<VEC>(out, b, total, y);
+    }
+  }
+}
+
+// A value per plane of hw > 1 elements.  Four planes have one counter block and are hw whole vectors of four, whatever hw is; a
+// vector meets two of them at most.  A block of threads takes a stretch of vectors, loads it, draws the counter blocks that it
+// meets, one a thread, into shared memory, and multiplies.  [256][512][7][7], both passes: 26 us, with a counter block for every
+// element 69, with a stored mask 40; [256][64][32][32] 48, 58 and 60 (floors 16 and 42).
+template <bool VEC, bool ADD>
+__global__ void __launch_bounds__(kThreads)
+dropout_planes_kernel(const float* a, const float* residual, float* out, size_t total, uint32_t hw, NrsFastDiv by_hw, const Draw draw, int accumulate) {
+  NRS_PDL_PROLOGUE();
+  constexpr uint32_t kStretch = kThreads * kUnroll;
+  __shared__ uint8_t s_kept[2][kStretch / 2 + 2];   // of every four planes met (at most one for two vectors, and a broken one): a bit for each
+  const size_t vectors = (total + 3) / 4;
+  const float* add = ADD ? (accumulate ? out : residual) : nullptr;
+  int turn = 0;                                     // (two stretches' bits: the one before may still be read)
+  for (size_t base = (size_t)blockIdx.x * kStretch; base < vectors; base += (size_t)gridDim.x * kStretch, turn ^= 1) {
+    float4 v[kUnroll], r[kUnroll];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (4 * b + j < total) out[4 * b + j] = e[j];
-      } else {
-        out[b] = y.x;
-      }
+    for (int u = 0; u < kUnroll; ++u) {
+      const size_t b = base + u * kThreads + threadIdx.x;
+      v[u] = r[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (b >= vectors) continue;
+      v[u] = load_four<VEC>(a, b, total);
+      if (ADD) r[u] = load_four<VEC>(add, b, total);
+    }
+    const size_t four0 = base >> 32 ? base / hw : (size_t)((uint32_t)base / hw);       // the four planes that the stretch starts in
+    const uint32_t at0 = (uint32_t)(base - four0 * hw);                                // and its first vector there
+    const uint32_t count = (uint32_t)min((size_t)kStretch, vectors - base);
+    auto four_of = [&](uint32_t at) { return hw >= kStretch ? (at >= hw ? 1u : 0u) : by_hw.div(at); };
+    const uint32_t fours = four_of(at0 + count - 1) + 1;
+    for (uint32_t i = threadIdx.x; i < fours; i += kThreads) {
+      uint32_t w[4];
+      nrs_rng::block(draw.seed, draw.first + four0 + i, w);
+      s_kept[turn][i] = (uint8_t)((w[0] > draw.last) | (w[1] > draw.last) << 1 | (w[2] > draw.last) << 2 | (w[3] > draw.last) << 3);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const uint32_t i = u * kThreads + threadIdx.x;
+      if (i >= count) continue;
+      const uint32_t at = at0 + i, four = four_of(at);
+      const uint64_t e = 4ull * (at - four * hw);                                      // the vector's first element among the four planes'
+      const uint32_t plane = (e >= hw) + (e >= 2ull * hw) + (e >= 3ull * hw), left = (uint32_t)min(4ull, (unsigned long long)((plane + 1ull) * hw - e));
+      const uint32_t kept = s_kept[turn][four] >> plane;
+      const float f = kept & 1 ? draw.kept : draw.dropped, g = kept & 2 ? draw.kept : draw.dropped;   // (left: elements of the first)
+      const float4 m = make_float4(f, left > 1 ? f : g, left > 2 ? f : g, left > 3 ? f : g);
+      float4 y = make_float4(v[u].x * m.x, v[u].y * m.y, v[u].z * m.z, v[u].w * m.w);
+      if (ADD) y = make_float4(fmaf(v[u].x, m.x, r[u].x), fmaf(v[u].y, m.y, r[u].y), fmaf(v[u].z, m.z, r[u].z), fmaf(v[u].w, m.w, r[u].w));
+      store_four<VEC>(out, base + i, total, y);
     }
   }
 }
@@ -248,19 +292,19 @@ static int dropout_pass(nrs_ctx* ctx, const char* who, const float* a, const flo
       const uint64_t left = ((uint64_t)1 << 32) - (uint32_t)draw.first;
       if ((total + 3) / 4 > left) part = (size_t)left * 4;
     }
-    const size_t groups = hw == 1 || (aligned && hw % 4 == 0) ? (part + 3) / 4 : part;
-    const size_t want = (groups + 4 * kThreads - 1) / (4 * kThreads), cap = (size_t)ctx->sm_count * 16;
+    const size_t want = ((part + 3) / 4 + 4 * kThreads - 1) / (4 * kThreads), cap = (size_t)ctx->sm_count * 16;
     const unsigned blocks = (unsigned)(want > cap ? cap : want);
-#define NRS_DROPOUT(FOURS_, VEC_)                                                                                                                     \
-  if (accumulate || residual)                                                                                                                         \
-    NRS_PDL_LAUNCH((dropout_kernel<FOURS_, VEC_, true>), blocks, kThreads, 0, ctx->stream, a, residual, out, part, (size_t)hw, draw, accumulate);      \
+    const bool add = accumulate || residual;
+#define NRS_DROPOUT(VEC_, ADD_)                                                                                                                       \
+  if (hw == 1)                                                                                                                                        \
+    NRS_PDL_LAUNCH((dropout_kernel<VEC_, ADD_>), blocks, kThreads, 0, ctx->stream, a, residual, out, part, draw, accumulate);                         \
   else                                                                                                                                                \
-    NRS_PDL_LAUNCH((dropout_kernel<FOURS_, VEC_, false>), blocks, kThreads, 0, ctx->stream, a, residual, out, part, (size_t)hw, draw, accumulate)
-    if (hw == 1 && aligned) {
+    NRS_PDL_LAUNCH((dropout_planes_kernel<VEC_, ADD_>), blocks, kThreads, 0, ctx->stream, a, residual, out, part, (uint32_t)hw, NrsFastDiv(hw), draw, accumulate)
+    if (aligned && add) {
       NRS_DROPOUT(true, true);
-    } else if (hw == 1) {
+    } else if (aligned) {
       NRS_DROPOUT(true, false);
-    } else if (aligned && hw % 4 == 0) {
+    } else if (add) {
       NRS_DROPOUT(false, true);
     } else {
       NRS_DROPOUT(false, false);
