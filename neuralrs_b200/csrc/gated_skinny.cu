@@ -44,7 +44,7 @@ struct Layout {
 
 struct Work {
   long total;            // slices of all tiles
-  int per_tile, tiles_n, chunks, slots_max;   // slices of a tile; column tiles, row chunks (fastest); shares of a tile at most
+  int per_tile, slots_max;   // slices of a tile; shares of a tile at most
   float* partial;        // [tile][share][N][128]
   __host__ __device__ long first_of(long cta, long ctas) const { return total * cta / ctas; }
   // The CTA that has slice i.
@@ -100,9 +100,9 @@ gated_skinny_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_const
     uint32_t s = 0, ph = 0, issued = 0;
     bool ok = true;
     const int tile0 = (int)(begin / wk.per_tile);   // (stepped along from here: a 64-bit division takes longer than a load's issue)
-    int at = (int)(begin - (long)tile0 * wk.per_tile), n0 = tile0 / wk.chunks * 64, chunk = tile0 % wk.chunks;
+    int at = (int)(begin - (long)tile0 * wk.per_tile), n0 = tile0 * 64;
     for (long i = begin; i < end; ++i) {
-      const int k0 = at * kSlice, m0 = chunk * N;
+      const int k0 = at * kSlice;
       if (!tc::mbar_wait_warp(&empty[s], ph ^ 1u)) { ok = false; break; }
       if (tc::elect_one()) {
         uint8_t* dst = smem + s * L::kSlot;
@@ -111,14 +111,14 @@ gated_skinny_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_const
         tma_load(dst + kWBytes / 4, &tm_g, &full[s], n0 + 32, k0);
         tma_load(dst + kWBytes / 2, &tm_u, &full[s], n0, k0);
         tma_load(dst + 3 * kWBytes / 4, &tm_u, &full[s], n0 + 32, k0);
-        tma_load(dst + kWBytes, &tm_x, &full[s], k0, m0);
+        tma_load(dst + kWBytes, &tm_x, &full[s], k0, 0);
       }
       __syncwarp();
       ++issued;
       if (++s == (uint32_t)L::kSlots) { s = 0; ph ^= 1u; }
       if (++at == wk.per_tile) {
         at = 0;
-        if (++chunk == wk.chunks) { chunk = 0; n0 += 64; }
+        n0 += 64;
       }
     }
     if (!ok) {   // loads under way still land here: wait for them, bounded
@@ -237,7 +237,7 @@ gated_skinny_kernel(const __grid_constant__ CUtensorMap tm_g, const __grid_const
 
 // h = act(a) u of the shares' sums.  A block: four rows of x, a tile's 64 columns.
 __global__ void __launch_bounds__(256)
-gated_shares_kernel(const Work wk, int rows /*of a chunk*/, long ctas, float* __restrict__ h, float* __restrict__ pre_gate, float* __restrict__ pre_up, int m, int n,
+gated_shares_kernel(const Work wk, int rows /*of a share*/, long ctas, float* __restrict__ h, float* __restrict__ pre_gate, float* __restrict__ pre_up, int m, int n,
                     int act) {
   NRS_PDL_PROLOGUE();
   const int tile = blockIdx.x, r = blockIdx.y * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
@@ -247,8 +247,8 @@ gated_shares_kernel(const Work wk, int rows /*of a chunk*/, long ctas, float* __
     s_shares = (int)(wk.owner(first + wk.per_tile - 1, ctas) - wk.owner(first, ctas)) + 1;
   }
   __syncthreads();
-  const int row = tile % wk.chunks * rows + r, col = tile / wk.chunks * 64 + c;
-  if (r >= rows || row >= m || col >= n) return;
+  const int col = tile * 64 + c;
+  if (r >= m || col >= n) return;
   const float* src = wk.partial + (long)tile * wk.slots_max * (rows * 128) + r * 128 + c;
   float a = 0.0f, u = 0.0f;
 #pragma unroll 4
@@ -256,7 +256,7 @@ gated_shares_kernel(const Work wk, int rows /*of a chunk*/, long ctas, float* __
     a += src[(long)s * (rows * 128)];
     u += src[(long)s * (rows * 128) + 64];
   }
-  const size_t at = (size_t)row * n + col;
+  const size_t at = (size_t)r * n + col;
   if (pre_gate) { pre_gate[at] = a; pre_up[at] = u; }
   h[at] = gated::act(a, act) * u;
 }
@@ -272,9 +272,7 @@ int run(nrs_ctx* ctx, const Shape& s, const float* x, const float* wg, const flo
   NRS_REQUIRE(ctx, ok, NRS_ERR_CUDA, "gated layer: cuTensorMapEncodeTiled failed (%d x %d x %d)", s.m, s.n, s.k);
   Work wk{};
   wk.per_tile = (s.k + kSlice - 1) / kSlice;
-  wk.tiles_n = (s.n + 63) / 64;
-  wk.chunks = (s.m + N - 1) / N;
-  const long tiles = (long)wk.tiles_n * wk.chunks;
+  const long tiles = (s.n + 63) / 64;
   wk.total = tiles * wk.per_tile;
   // At least two slices a CTA.
   const long ctas = std::min<long>(ctx->sm_count, std::max<long>(1, wk.total / 2)), least = wk.total / ctas;
@@ -293,8 +291,7 @@ int run(nrs_ctx* ctx, const Shape& s, const float* x, const float* wg, const flo
   NrsProfScope prof(ctx, NRS_PROF_GEMM, 4.0 * s.m * s.n * s.k);
   NRS_PDL_LAUNCH(gated_skinny_kernel<N>, (unsigned)ctas, kThreads, L::kBytes, ctx->stream, g, u, t, wk, err);
   NRS_LAUNCHED(ctx);
-  const int rows = std::min(N, s.m);
-  NRS_PDL_LAUNCH(gated_shares_kernel, dim3((unsigned)tiles, (unsigned)((rows + 3) / 4)), 256, 0, ctx->stream, wk, N, ctas, h, pg, pu, s.m, s.n, s.act);
+  NRS_PDL_LAUNCH(gated_shares_kernel, dim3((unsigned)tiles, (unsigned)((s.m + 3) / 4)), 256, 0, ctx->stream, wk, N, ctas, h, pg, pu, s.m, s.n, s.act);
   NRS_LAUNCHED(ctx);
   return NRS_OK;
 }
@@ -303,7 +300,7 @@ int run(nrs_ctx* ctx, const Shape& s, const float* x, const float* wg, const flo
 
 int nrs_gated_skinny_fwd(nrs_ctx* ctx, const Shape& s, const float* x, const float* wg, const float* wu, float* h, float* pre_gate, float* pre_up) {
   const bool whole = s.n % 4 == 0 && s.k % 4 == 0 && (((uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu) & 15) == 0;   // TMA's strides and addresses
-  if (ctx->math_mode != NRS_MATH_3XTF32 || !whole || !tc::tensor_map_encoder() || (long)s.n * ((s.m + 15) / 16) > (1L << 28)) return NRS_ERR_UNSUPPORTED;
+  if (ctx->math_mode != NRS_MATH_3XTF32 || !whole || !tc::tensor_map_encoder() || s.m > 128 || s.n > (1 << 28)) return NRS_ERR_UNSUPPORTED;
   if (s.m <= 16) return run<16>(ctx, s, x, wg, wu, h, pre_gate, pre_up);
   if (s.m <= 32) return run<32>(ctx, s, x, wg, wu, h, pre_gate, pre_up);
   if (s.m <= 64) return run<64>(ctx, s, x, wg, wu, h, pre_gate, pre_up);
