@@ -74,18 +74,32 @@ int nrs_workspace(nrs_ctx* ctx, size_t bytes, void** out) {
   return st;
 }
 
+// Is the context's stream being captured?  (On the legacy stream, beside a capture, even asking fails.  That error is told here,
+// ahead of a launch that would end the other capture, and not left to the next check of a launch.)
+static int is_capturing(nrs_ctx* ctx, bool* yes) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(ctx->stream, &status);
+  *yes = e == cudaSuccess && status != cudaStreamCaptureStatusNone;
+  if (e == cudaSuccess) return NRS_OK;
+  (void)cudaGetLastError();
+  return nrs_fail(ctx, NRS_ERR_CUDA, "the context's stream cannot be used now: %s", cudaGetErrorString(e));
+}
+
 int nrs_ws_slot(nrs_ctx* ctx, int slot, size_t bytes, void** out) {
+  *out = nullptr;
   if (slot < 0 || slot >= NRS_WS_COUNT) return nrs_fail(ctx, NRS_ERR_ARG, "workspace: bad slot %d", slot);
+  bool capturing = false;
+  int st = is_capturing(ctx, &capturing);
+  if (st != NRS_OK) return st;
   if (bytes > ctx->ws_slot_bytes[slot] && ctx->ws_slot_captured[slot]) {
     ctx->ws_kept.emplace_back(ctx->ws_slot[slot], ctx->ws_slot_bytes[slot]);
     ctx->ws_slot[slot] = nullptr;
     ctx->ws_slot_bytes[slot] = 0;
     ctx->ws_slot_captured[slot] = false;
   }
-  const int st = grow_block(ctx, "workspace slot", bytes, &ctx->ws_slot[slot], &ctx->ws_slot_bytes[slot]);
+  st = grow_block(ctx, "workspace slot", bytes, &ctx->ws_slot[slot], &ctx->ws_slot_bytes[slot]);
   *out = ctx->ws_slot[slot];
-  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-  if (st == NRS_OK && cudaStreamIsCapturing(ctx->stream, &capturing) == cudaSuccess && capturing != cudaStreamCaptureStatusNone) ctx->ws_slot_captured[slot] = true;
+  if (st == NRS_OK && capturing) ctx->ws_slot_captured[slot] = true;
   return st;
 }
 
@@ -123,9 +137,10 @@ int nrs_range_new(nrs_ctx* ctx, NrsRange** out, int count) {
     pool.captured = (NrsRange*)mem;
     pool.captured_left = NrsRangePool::kCaptured;
   }
-  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-  NRS_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capturing));
-  if (capturing != cudaStreamCaptureStatusNone) {
+  bool capturing = false;
+  const int asked = is_capturing(ctx, &capturing);
+  if (asked != NRS_OK) return asked;
+  if (capturing) {
     *out = pool.captured;
     pool.captured += count;
     pool.captured_left -= count;
