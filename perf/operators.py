@@ -13,6 +13,7 @@ products run in its default precision.
 from __future__ import annotations
 
 import math
+import threading
 
 import numpy as np
 import torch
@@ -277,19 +278,20 @@ def _gated(s):
 
 # ------------------------------------------------------------------------------------------------ the framework's calls
 
-_handle = []
+_here = threading.local()   # (which stream is the current one goes by the thread, too)
 
 
 def _framework():
-    """The library and a context on the program's own stream, made once."""
-    if not _handle:
+    """The library and a context on the program's own stream, made once; the stream waits for the inputs made before."""
+    if not hasattr(_here, "handle"):
         from neuralrs_b200 import _lib, cuda
         stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
         torch.cuda.set_stream(stream)
         ctx = cuda.Context(torch.cuda.current_device())
         ctx.set_stream(stream.cuda_stream)
-        _handle.extend([_lib.lib(), ctx, stream, _lib.check, {"gelu": _lib.ACT_GELU, "silu": _lib.ACT_SILU}])
-    return _handle
+        _here.handle = [_lib.lib(), ctx, stream, _lib.check, {"gelu": _lib.ACT_GELU, "silu": _lib.ACT_SILU}]
+    return _here.handle
 
 
 def _p(t, at=0):
