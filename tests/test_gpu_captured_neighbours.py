@@ -48,3 +48,70 @@ def test_a_call_on_the_legacy_stream_beside_a_capture(gpu_ctx):
     torch.cuda.synchronize()
     assert torch.equal(h, want)
     ctx.close()
+
+
+def test_gradients_and_replays_beside_a_capture(gpu_ctx, oracle32):
+    """An eager block's gradients are, bit for bit, those of the same block with nothing captured between its passes; and the
+    replayed calls leave what the same calls leave eagerly, on other inputs too."""
+    from neuralrs_b200.cuda import backward_graph
+    from neuralrs_b200.cuda import runtime as gpu
+    from .test_gpu_modern_block import Block, formulas, parameters, P, SEED
+    rng = np.random.default_rng(1)
+    p = parameters(rng, 60, 32, 2, 64)
+    ids, labels = rng.integers(0, 60, (2, 8)), rng.integers(0, 60, 16)
+    l, ctx, s = _lib.lib(), cuda.Context(0), torch.cuda.Stream()
+    ctx.set_stream(s.cuda_stream)
+
+    def captured():
+        with torch.cuda.stream(s):
+            x, dh = torch.randn(64, 32, device="cuda"), torch.randn(64, 64, device="cuda")
+            wg, wu = torch.randn(32, 64, device="cuda"), torch.randn(32, 64, device="cuda")
+            h, a, u = (torch.empty(64, 64, device="cuda") for _ in range(3))
+            dx, dwg, dwu = torch.empty_like(x), torch.empty_like(wg), torch.empty_like(wu)
+
+            def both():
+                q = lambda *ts: [t.data_ptr() for t in ts]
+                _lib.check(ctx.h, l.nrs_gated_linear_fwd(ctx.h, *q(x, wg, wu, h, a, u), 64, 64, 32, SILU))
+                _lib.check(ctx.h, l.nrs_gated_linear_bwd(ctx.h, *q(x, wg, wu, a, u, dh, dx, dwg, dwu), 64, 64, 32, SILU, 0, 0))
+            both()
+            s.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                both()
+            for scale in (1.0, 30.0):
+                for t in (x, wg, wu, dh):
+                    t.normal_().mul_(scale)
+                for t in (h, a, u, dx, dwg, dwu):
+                    t.fill_(float("nan"))
+                g.replay()
+                s.synchronize()
+                got = [t.clone() for t in (h, a, u, dx, dwg, dwu)]
+                both()
+                s.synchronize()
+                for t, want in zip(got, (h, a, u, dx, dwg, dwu)):
+                    assert torch.equal(t, want)
+                pre = [x.double() @ w.double() for w in (wg, wu)]
+                want = torch.nn.functional.silu(pre[0]) * pre[1]
+                assert float((got[0] - want).norm() / want.norm()) < 1e-5
+        return g
+
+    def step(between):
+        _lib.check(gpu_ctx.h, l.nrs_rng_seed(gpu_ctx.h, SEED))
+        block = Block(p, 2, True, 8)
+        logits = block.forward(ids)
+        kept = between()
+        z = gpu.to_host(logits).reshape(16, 60).astype(np.float64)
+        e = np.exp(z - z.max(1, keepdims=True))
+        gpu.set_grad(logits, ((e / e.sum(1, keepdims=True) - np.eye(60)[labels]) / 16).astype(np.float32))
+        backward_graph(logits)
+        del kept
+        return {k: gpu.read_grad(v) for k, v in block.n.items()}
+
+    alone, beside = step(lambda: None), step(captured)
+    n = 2 * 8 * 32
+    masks = [oracle32.dropout_mask(n, P, SEED, i * ((n + 3) // 4)).astype(np.float64) for i in range(2)]
+    _, want = formulas(p, ids, labels, 2, True, masks)
+    for k in alone:
+        assert np.array_equal(alone[k], beside[k]), k
+        assert np.linalg.norm(alone[k].ravel() - want[k].ravel()) <= 1e-4 * np.linalg.norm(want[k]), k
+    ctx.close()
