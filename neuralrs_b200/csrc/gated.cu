@@ -123,7 +123,7 @@ gated_few_kernel(const float* __restrict__ x, const float* __restrict__ wg, cons
 
 int few_rows(nrs_ctx* ctx, const Shape& s, const float* x, const float* wg, const float* wu, float* h, float* pg, float* pu) {
   const bool vec = s.n % 4 == 0 && (((uintptr_t)wg | (uintptr_t)wu) & 15) == 0;
-  const int blocks = (s.n + kCols - 1) / kCols;
+  const int blocks = (s.n - 1) / kCols + 1;   // (n up to the last that an int counts)
   int shares = 1;   // until there are two blocks an SM, or a share of k is two loads of a warp
   while (shares < 8 && blocks * shares < 2 * ctx->sm_count && s.k / (2 * shares) >= 256) shares *= 2;
   const int per = (s.k + shares - 1) / shares;

@@ -398,9 +398,9 @@ int run(nrs_ctx* ctx, const Planes& A, const Planes& B, GatedPolicy<P> pol, int 
 
 bool applies(const nrs_ctx* ctx, const Shape& s) {
   // (from 16 rows on, as the ungated products; the staging passes count eights in 32 bits)
+  if (s.n > (1 << 24) || s.k > (1 << 24)) return false;
   const uint64_t m = s.m, n = round64(s.n), k = round64(s.k), most = 1ull << 33;
-  return ctx->math_mode == NRS_MATH_3XTF32 && tc::tensor_map_encoder() && s.m >= 16 && s.n >= 32 && s.k >= 32 && s.n <= (1 << 24) && s.k <= (1 << 24) &&
-         m * n <= most && m * k <= most && k * n <= most;
+  return ctx->math_mode == NRS_MATH_3XTF32 && tc::tensor_map_encoder() && s.m >= 16 && s.n >= 32 && s.k >= 32 && m * n <= most && m * k <= most && k * n <= most;
 }
 
 }  // namespace

@@ -1,8 +1,11 @@
 """Gated feed-forward layers at the limits of what they are given: matrices of very different magnitudes side by side, gates far from
 zero.  Against the formulas in 64 bits."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
+from neuralrs_b200 import _lib
 from .conftest import rel_l2
 from .gpu_util import Dev, call
 
@@ -182,3 +185,19 @@ def test_closed_gates_of_the_lowest_value(gpu_ctx):
     got, want = backward(gpu_ctx, x, wg, wu, a, u, dh), formulas(x, wg, wu, dh, a, u)
     for name in got:
         assert rel_l2(got[name], want[name]) <= 3 * 8 * U * 1.2, name
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 4])   # a column a lane, and four
+def test_as_many_columns_as_an_int_counts(gpu_ctx, n):
+    l, w, h = _lib.lib(), Dev(gpu_ctx, shape=(n,), zero=True), Dev(gpu_ctx, shape=(n,))
+    ones, at = np.ones(40, np.float32), lambda d, i: C.c_void_p(d.ptr.value + 4 * i)
+    spots = [0, n // 2, n - 40]
+    for i in spots:
+        _lib.check(gpu_ctx.h, l.nrs_h2d(gpu_ctx.h, at(w, i), C.c_void_p(ones.ctypes.data), ones.nbytes))
+    call(gpu_ctx, "nrs_gated_linear_fwd", Dev(gpu_ctx, np.full((1, 1), 2.0, np.float32)), w, w, h, None, None, 1, n, 1, 1)   # relu(2 w) * 2 w
+    for i in spots:
+        got = np.empty(48, np.float32)
+        first = max(0, min(i - 4, n - 48))
+        _lib.check(gpu_ctx.h, l.nrs_d2h(gpu_ctx.h, C.c_void_p(got.ctypes.data), at(h, first), got.nbytes))
+        inside = (first + np.arange(48) >= i) & (first + np.arange(48) < i + 40)
+        assert np.array_equal(got, np.where(inside, 4.0, 0.0).astype(np.float32))
