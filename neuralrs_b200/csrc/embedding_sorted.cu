@@ -98,7 +98,7 @@ struct Plan {
   __host__ __device__ int piece() const { return kSumWarps * per_warp; }
 };
 Plan plan_of(int tokens, int dim, int vocab, int sm_count) {
-  Plan p{tokens, dim, vocab, 0, (dim + kSlab - 1) / kSlab, 32, 0};
+  Plan p{tokens, dim, vocab, 0, (dim - 1) / kSlab + 1, 32, 0};
   p.range = std::min(kMaxRange, (vocab + sm_count - 1) / sm_count);
   while (p.per_warp > 4 && (long)((tokens + p.piece() - 1) / p.piece()) * p.slabs < kFillBlocks) p.per_warp /= 2;
   p.pieces = (tokens + p.piece() - 1) / p.piece();
