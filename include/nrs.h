@@ -177,9 +177,10 @@ int nrs_bmm(nrs_ctx* ctx, int trans_a, int trans_b, int batch, int m, int n, int
 
 /* Gated feed-forward layer (no reference counterpart; the gated form of src/cuda/nn/transformer_block.rs:37):
  *   h[m,n] = act(x[m,k] . w_gate[k,n]) * (x . w_up[k,n])
- * both projections, the activation (any nrs_act; NONE: a product of two projections) and the product in one kernel.
+ * act: any nrs_act (NONE: a product of two projections).
  * pre_gate, pre_up (both or neither): [m,n], the projections, which the backward pass reads.
- * Backward: dx (+)=, and dw_gate, dw_up (+)= (both or neither); dx and the pair may be NULL.
+ * Backward: dx (+)=, and dw_gate, dw_up (+)= (both or neither); dx and the pair may be NULL.  SiLU and GELU are 0, and their
+ * slopes 0 or 1, where their exponential leaves f32's normal range.
  * 3xTF32 mode, with the error of an f32 product.  Forward: up to 4 rows, and small layers of up to 15, in f32; the
  * others up to 32 rows, and up to 128 where k >= 256, three TF32 products of operands split in two, summed in f32 every 32
  * values (n, k multiples of 4 and 16-byte addresses); else, and backward, f16 pairs in accumulation chains of 256 values, added

@@ -140,7 +140,8 @@ int nrs_op_qk_norm_rotary(nrs_node* q, nrs_node* k, nrs_node* gamma_q, nrs_node*
                           const int32_t* positions_host, int64_t heads_q, int64_t heads_k, int interleaved, float eps,
                           nrs_node** q_out, nrs_node** k_out);
 /* nrs_op_mha whose queries and keys go through nrs_op_qk_norm_rotary (gamma_q, gamma_k: [d / num_heads]) on their way
- * from the projections to the scores. */
+ * from the projections to the scores.  The projections are three products, and attention runs as in nrs_op_attention_batch:
+ * not over operand planes, which nrs_op_mha takes for longer sequences. */
 int nrs_op_mha_rotary(nrs_node* x, nrs_node* w_q, nrs_node* w_k, nrs_node* w_v, nrs_node* w_o, nrs_node* gamma_q,
                       nrs_node* gamma_k, nrs_node* table, int64_t num_heads, int interleaved, float eps, int causal,
                       nrs_node** out);

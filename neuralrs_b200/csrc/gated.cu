@@ -146,7 +146,9 @@ int few_rows(nrs_ctx* ctx, const Shape& s, const float* x, const float* wg, cons
   return NRS_OK;
 }
 
-// Where the tensor-core form without a pass over the weights is the fastest (us; few rows, that one, staged operands):
+// Where the tensor-core form without a pass over the weights is the fastest (us; few rows, that one, staged operands).  Up to 4
+// rows stay in f32 and one launch: ahead on smaller layers; with the weights out of L2 a tenth behind at 2048 x 5504 and a sixth at
+// 8192 x 5504.
 //   rows  k x n         few   this  staged        rows  k x n        this  staged
 //   4     2048 x 5504   25.0  24.1                 16   2048 x 5504   24.9  78.4
 //   8     2048 x 5504   55.2  24.7                128   2048 x 5504   52.8  80.1

@@ -13,9 +13,12 @@
 // columns on 148 SMs would idle two in five): a stretch's share of a tile goes to scratch, and a second launch adds the shares
 // up in order, applies the activation and multiplies.
 //
-// A slice costs shared memory 16 KB in, 16 KB out and in again for the split, and 32 KB for the UMMAs' reads, about 730 clocks;
-// memory brings a slice in 710 when all SMs ask.  2048 -> 5504, 90 MB of weights (floor 14 us): 16 rows 25 us, 64 rows 34 us;
-// with one group of splitting warps, which then also drained, 31 and 41 us; measuring and staging the weights first 78 us.
+// 2048 -> 5504, 90 MB of weights (floor 14 us): 16 rows 25 us, 64 rows 34 us; with one group of splitting warps, which then also
+// drained, 31 and 41 us; measuring and staging the weights first 78 us.  A slice costs shared memory 16 KB in, 16 KB out and in
+// again for the split, and 32 KB for the UMMAs' reads, about 730 clocks by count, and memory brings one in 710 when all SMs
+// ask.  Taken from 2048 and 8192 values of k it costs 0.43 us at 16 rows (some 800 clocks), 0.62 at 64 and 1.0 at 128, where
+// x's slice, as large as the weights', is split too and leaves the ring three slots.  An SM has 37 of them here; what is left,
+// 9, 10 and 15 us, is two launches: the first one's start and the filling of its ring, the shares and their sum.
 #include <algorithm>
 
 #include "gated.h"

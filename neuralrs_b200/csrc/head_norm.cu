@@ -10,7 +10,8 @@
 //
 // Bound by memory: 8 bytes a feature forward, 12 backward.  A row is held in the registers of L neighbouring lanes, eight
 // features each in two 16-byte accesses, placed so that a lane holds both members of its pairs: nothing but the row sum
-// crosses lanes.  A warp works on one token at a time: the angles are looked up once for all its heads.
+// crosses lanes.  A warp's rows are heads side by side, of one token or of several; each looks up its own position and angles,
+// which the caches keep for the token's other heads.
 #include <algorithm>
 
 #include "igemm_problems.cuh"

@@ -509,7 +509,8 @@ class nn:
 
     class MultiHeadAttention:
         """src/cuda/nn/multihead.rs:20-85 (weights [d,d], no biases).  head_norm (an nn.HeadNorm, an extension): norms and
-        rotations of the projected queries and keys."""
+        rotations of the projected queries and keys; its weights are among the parameters, behind w_o.  With it the
+        projections are three products and attention does not run over operand planes."""
 
         def __init__(self, w_q, w_k, w_v, w_o, d_model: int, num_heads: int, causal: bool = False, head_norm=None):
             self.w_q, self.w_k, self.w_v, self.w_o = w_q, w_k, w_v, w_o
